@@ -7,6 +7,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libpsvae_hip.so')
 SOURCES = ['gemm.hip', 'fused_layer.hip', 'graph_kernels.hip', 'head_kernels.hip', 'gru.hip', 'step.hip', 'inference.hip', 'collate_device.hip', 'capi.hip', 'profiler.hip', 'rng.hip', 'collate.cpp']
+# No packed fp32 instructions (v_pk_add/mul/fma_f32, which hipcc forms from ordinary float code): some of their forms have
+# given wrong results now and then on these GPUs.  The host pass of hipcc does not know the feature and says so.
+DEVICE_FLAGS = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 HEADERS = ['psvae_internal.h', 'fused_device.h', os.path.join('..', '..', 'include', 'psvae.h')]
 
 
@@ -27,7 +30,8 @@ def build(force=False, verbose=False):
     os.makedirs(os.path.join(HERE, 'build'), exist_ok=True)
     for src in SOURCES:
         obj = os.path.join(HERE, 'build', src.rsplit('.', 1)[0] + '.o')
-        cmd = [hipcc, '--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-c', os.path.join(CSRC, src), '-o', obj]
+        cmd = [hipcc, '--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', *(DEVICE_FLAGS if src.endswith('.hip') else []), '-c',
+               os.path.join(CSRC, src), '-o', obj]
         if verbose:
             print(' '.join(cmd))
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
