@@ -56,6 +56,15 @@ enum {
 const char* psvae_strerror(int code);
 int psvae_abi_version(void);
 
+/* element types of the sequence-block operators' activations (their parameters, states and statistics are fp32) */
+enum { PSVAE_F32 = 0, PSVAE_BF16 = 1, PSVAE_F16 = 2 };
+/* their flags */
+enum {
+    PSVAE_SEQ_SILU = 1,         /* convolution: SiLU behind the filter */
+    PSVAE_SEQ_SOFTPLUS = 2,     /* scan: delta = softplus(dt + dt_bias) instead of dt + dt_bias */
+    PSVAE_SEQ_ZERO_OUTSIDE = 4  /* write zeros to the output rows that no sequence holds instead of leaving them as they were */
+};
+
 /* ---- kernel-selection options (no counterpart in the reference) -------------
  * Where the library chooses between two forms of a kernel by problem size, the choice can be forced: value -1 =
  * the library's own choice (the default), otherwise as listed.  An option is read on every call, so it can be
@@ -75,6 +84,7 @@ int psvae_abi_version(void);
  *   gru_tiles      1 / 2 / 4: sequence tiles a workgroup of the multi-CU recurrence steps together
  *   gru_spin_ticks bound of a wait inside the multi-CU recurrence in ticks of 10 ns (default 2 s); 0: give up at
  *                  once, which exercises the redo on the single-CU kernels
+ *   scan_chunks    1 .. 64: pieces of the time axis that the selective scan runs beside each other
  * psvae_option_set / _get return PSVAE_E_SHAPE for an unknown name; psvae_option_name(i) enumerates the names
  * (NULL past the last). */
 int psvae_option_set(const char* name, int value);
@@ -439,6 +449,82 @@ int psvae_gru_forward_stamped(const float* gi, const float* h0, const float* whh
 int psvae_softmax_ce_forward(const float* logits, int ld, const int32_t* target, int target_stride,
                              int target_offset, int rows_per_group, int rows, int classes, int ignore_index,
                              float* row_loss, float* lse, void* stream);
+
+/* ---- sequence-block operators (no counterpart in the reference, whose piece decoder is the GRU above): what a
+ * state-space piece decoder is built from, beside psvae_linear_* and psvae_gru_*.  Activations are matrices of `dtype`
+ * (PSVAE_F32 / _BF16 / _F16) whose rows may lie `ld` elements apart; arithmetic, sums and statistics are fp32 and a
+ * result is rounded once, where it is stored.  Any sizes, strides and element-aligned addresses are accepted; rows of
+ * every operand that begin on 16 bytes and hold whole 16-byte vectors are faster.  Outputs must not overlap inputs
+ * unless stated.  No atomics: the same call gives the same bits.
+ *
+ * Packed sequences (convolution and scan): T rows; with `seq_off` (DEVICE int32 [S+1], non-decreasing) sequence s holds
+ * rows seq_off[s] .. seq_off[s+1]-1, lengths of 0 included; without it (NULL) S sequences of T / S rows each.  Rows
+ * before seq_off[0] and from seq_off[S] on belong to no sequence: outputs and input gradients there are left as they
+ * were, or zeroed with PSVAE_SEQ_ZERO_OUTSIDE, and add nothing to any sum.  The offsets are not checked (they are in
+ * device memory); whatever they hold, no access leaves the T rows. */
+
+/* Layer norm over the last dimension: y = (x - mean) / sqrt(var + eps) * weight + bias, var = the mean squared distance
+ * from the mean; weight and bias [width] may be NULL (1 and 0).  mean and rstd [rows], what backward reads, may be NULL.
+ * Backward: dx (NULL: not wanted), d_weight and d_bias [width] (NULL: not wanted; with either, scratch of
+ * psvae_layer_norm_scratch_bytes, 16-byte aligned).  1 <= width <= 2^23. */
+int psvae_layer_norm_forward(const void* x, int64_t ldx, const float* weight, const float* bias, void* y, int64_t ldy,
+                             float* mean, float* rstd, int64_t rows, int width, float eps, int dtype, void* stream);
+size_t psvae_layer_norm_scratch_bytes(int64_t rows, int width);
+int psvae_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* weight,
+                              const float* mean, const float* rstd, void* dx, int64_t lddx, float* d_weight,
+                              float* d_bias, int64_t rows, int width, int dtype, void* scratch, size_t scratch_bytes,
+                              void* stream);
+
+/* Short causal convolution, one filter of W taps a channel (1 <= W <= 8, weight [D, W], bias [D] or NULL):
+ *   y[t, d] = act(bias[d] + sum_k weight[d, k] x[t - W + 1 + k, d]),   act = SiLU with PSVAE_SEQ_SILU, else nothing.
+ * The rows in front of a sequence are state[s] ([S, W-1, D] of `dtype`, the inputs before it, oldest first), or zero
+ * (NULL).  state_out (or NULL; not `state` itself) receives the same of the sequence's end.  Backward takes no gradient
+ * for the states; scratch as above when d_weight [D, W] or d_bias is wanted.
+ * _step: one row for each of S sequences; reads `state`, writes the shifted state to `state_out`, which may be `state`. */
+int psvae_causal_conv_forward(const void* x, int64_t ldx, const float* weight, const float* bias, void* y, int64_t ldy,
+                              const int32_t* seq_off, const void* state, void* state_out, int64_t T, int S, int D,
+                              int W, int dtype, int flags, void* stream);
+size_t psvae_causal_conv_scratch_bytes(int64_t T, int D, int W, int dtype);
+int psvae_causal_conv_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* weight,
+                               const float* bias, void* dx, int64_t lddx, float* d_weight, float* d_bias,
+                               const int32_t* seq_off, const void* state, int64_t T, int S, int D, int W, int dtype,
+                               int flags, void* scratch, size_t scratch_bytes, void* stream);
+int psvae_causal_conv_step(const void* x, int64_t ldx, const void* state, void* state_out, const float* weight,
+                           const float* bias, void* y, int64_t ldy, int S, int D, int W, int dtype, int flags,
+                           void* stream);
+
+/* Selective scan: D channels with N states each (1 <= N <= 64), G groups of D / G neighbouring channels sharing B and C:
+ *   delta = softplus(dt + dt_bias)  (PSVAE_SEQ_SOFTPLUS; otherwise dt + dt_bias)
+ *   h[t, d, n] = exp(delta[t, d] A[d, n]) h[t-1, d, n] + delta[t, d] x[t, d] B[t, g, n]
+ *   y[t, d] = (sum_n C[t, g, n] h[t, d, n] + skip[d] x[t, d]) * silu(z[t, d])
+ * x, dt, z [T, D], B and C [T, G N] of `dtype`; A [D, N], skip [D], dt_bias [D] and the states h0, hT [S, D, N] fp32,
+ * contiguous.  z, skip, dt_bias, h0 (and, as outputs, hT) may be NULL.
+ * _forward: with `saved` (psvae_selective_scan_saved_bytes, 16-byte aligned; the state every 16 rows) a backward pass can
+ *   follow.  scratch: psvae_selective_scan_scratch_bytes(.., backward = 0), 0 where the time axis is not cut.
+ * _backward: given dy (gradient of y) and dhT (of hT, or NULL), writes every gradient of psvae_scan_grads; dz may be NULL
+ *   without z, and d_skip, d_dt_bias and dh0 where they are not wanted.  Same `a` and `saved` as the forward call.
+ *   scratch: psvae_selective_scan_scratch_bytes(.., backward = 1), 16-byte aligned.
+ * _step: one row for each of S sequences (T = S, no seq_off): reads h0, writes hT, which may be h0. */
+typedef struct psvae_scan {
+    const void *x, *dt, *B, *C, *z;
+    int64_t ldx, lddt, ldb, ldc, ldz;
+    const float *A, *skip, *dt_bias, *h0;
+    const int32_t* seq_off;
+    int64_t T;
+    int32_t S, D, G, N, dtype, flags;
+} psvae_scan;
+typedef struct psvae_scan_grads {
+    void *dx, *ddt, *dB, *dC, *dz;
+    int64_t lddx, ldddt, lddb, lddc, lddz;
+    float *dA, *d_skip, *d_dt_bias, *dh0;
+} psvae_scan_grads;
+size_t psvae_selective_scan_scratch_bytes(int64_t T, int S, int D, int G, int N, int backward);
+size_t psvae_selective_scan_saved_bytes(int64_t T, int S, int D, int G, int N);
+int psvae_selective_scan_forward(const psvae_scan* a, void* y, int64_t ldy, float* hT, void* saved, void* scratch,
+                                 size_t scratch_bytes, void* stream);
+int psvae_selective_scan_backward(const psvae_scan* a, const void* saved, const void* dy, int64_t lddy, const float* dhT,
+                                  const psvae_scan_grads* g, void* scratch, size_t scratch_bytes, void* stream);
+int psvae_selective_scan_step(const psvae_scan* a, void* y, int64_t ldy, float* hT, void* stream);
 
 /* ---- host-side batching (bit-exact integer work, no GPU involved) ----------
  * psvae_collate_pairs = the edge / pair enumeration loop of process_step3

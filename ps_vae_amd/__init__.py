@@ -10,7 +10,7 @@ def __getattr__(name):
     if name in ('PSVAEModel',):
         from .model import PSVAEModel
         return PSVAEModel
-    if name in ('Encoder', 'VAEPieceDecoder', 'Predictor', 'MLP'):
+    if name in ('Encoder', 'VAEPieceDecoder', 'Predictor', 'MLP', 'LayerNorm', 'SSMBlock'):
         from . import modules
         return getattr(modules, name)
     if name in ('BPEMolDataset', 'PackedMolDataset', 'get_dataloader', 'to_device', 'NativeBatch'):

@@ -92,6 +92,20 @@ class MolStore(C.Structure):
         'in_edge_off', 'in_rowptr_loc', 'in_nbr', 'in_nbr_type', 'piece_off', 'pieces', 'props')] + [('n_props_all', i32)])
 
 
+class Scan(C.Structure):
+    _fields_ = ([(k, vp) for k in ('x', 'dt', 'B', 'C', 'z')] + [(k, i64) for k in ('ldx', 'lddt', 'ldb', 'ldc', 'ldz')] +
+                [(k, vp) for k in ('A', 'skip', 'dt_bias', 'h0', 'seq_off')] + [('T', i64)] +
+                [(k, i32) for k in ('S', 'D', 'G', 'N', 'dtype', 'flags')])
+
+
+class ScanGrads(C.Structure):
+    _fields_ = ([(k, vp) for k in ('dx', 'ddt', 'dB', 'dC', 'dz')] + [(k, i64) for k in ('lddx', 'ldddt', 'lddb', 'lddc', 'lddz')] +
+                [(k, vp) for k in ('dA', 'd_skip', 'd_dt_bias', 'dh0')])
+
+
+F32, BF16, F16 = 0, 1, 2
+SEQ_SILU, SEQ_SOFTPLUS, SEQ_ZERO_OUTSIDE = 1, 2, 4
+
 _lib = None
 
 
@@ -175,6 +189,23 @@ def lib():
     L.psvae_collate_device.argtypes = [P(MolStore), vp, C.c_int, C.c_int, i64, i64, C.c_int, i64, C.c_double, C.c_uint64,
                                        C.c_uint64, C.c_int, C.c_int, C.c_int, C.c_int, vp, C.c_int, vp, i64, vp, vp, vp,
                                        vp, sz, vp]
+    ci = C.c_int
+    L.psvae_layer_norm_forward.argtypes = [vp, i64, vp, vp, vp, i64, vp, vp, i64, ci, f32, ci, vp]
+    L.psvae_layer_norm_scratch_bytes.restype = sz
+    L.psvae_layer_norm_scratch_bytes.argtypes = [i64, ci]
+    L.psvae_layer_norm_backward.argtypes = [vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, i64, ci, ci, vp, sz, vp]
+    L.psvae_causal_conv_forward.argtypes = [vp, i64, vp, vp, vp, i64, vp, vp, vp, i64, ci, ci, ci, ci, ci, vp]
+    L.psvae_causal_conv_scratch_bytes.restype = sz
+    L.psvae_causal_conv_scratch_bytes.argtypes = [i64, ci, ci, ci]
+    L.psvae_causal_conv_backward.argtypes = [vp, i64, vp, i64, vp, vp, vp, i64, vp, vp, vp, vp, i64, ci, ci, ci, ci, ci, vp, sz, vp]
+    L.psvae_causal_conv_step.argtypes = [vp, i64, vp, vp, vp, vp, vp, i64, ci, ci, ci, ci, ci, vp]
+    L.psvae_selective_scan_scratch_bytes.restype = sz
+    L.psvae_selective_scan_scratch_bytes.argtypes = [i64, ci, ci, ci, ci, ci]
+    L.psvae_selective_scan_saved_bytes.restype = sz
+    L.psvae_selective_scan_saved_bytes.argtypes = [i64, ci, ci, ci, ci]
+    L.psvae_selective_scan_forward.argtypes = [P(Scan), vp, i64, vp, vp, vp, sz, vp]
+    L.psvae_selective_scan_backward.argtypes = [P(Scan), vp, vp, i64, vp, P(ScanGrads), vp, sz, vp]
+    L.psvae_selective_scan_step.argtypes = [P(Scan), vp, i64, vp, vp]
     L.psvae_profile_enable.argtypes = [C.c_int]
     L.psvae_profile_num_classes.restype = C.c_int
     L.psvae_profile_class_name.restype = C.c_char_p
@@ -199,6 +230,10 @@ EXPORTS = (
     'psvae_segment_pool_forward',
     'psvae_gru_exchange_bytes', 'psvae_gru_forward', 'psvae_gru_forward_stamped', 'psvae_gru_backward', 'psvae_softmax_ce_forward', 'psvae_collate_pairs', 'psvae_gather_molecules',
     'psvae_pack_bound', 'psvae_pack_batch', 'psvae_collate_device_layout', 'psvae_collate_device_scratch_bytes',
+    'psvae_layer_norm_forward', 'psvae_layer_norm_scratch_bytes', 'psvae_layer_norm_backward', 'psvae_causal_conv_forward',
+    'psvae_causal_conv_scratch_bytes', 'psvae_causal_conv_backward', 'psvae_causal_conv_step',
+    'psvae_selective_scan_scratch_bytes', 'psvae_selective_scan_saved_bytes', 'psvae_selective_scan_forward',
+    'psvae_selective_scan_backward', 'psvae_selective_scan_step',
     'psvae_collate_device', 'psvae_profile_enable', 'psvae_profile_num_classes',
     'psvae_profile_class_name', 'psvae_profile_collect', 'psvae_profile_event_overhead_ms')
 

@@ -6,11 +6,11 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libpsvae_hip.so')
-SOURCES = ['gemm.hip', 'fused_layer.hip', 'graph_kernels.hip', 'head_kernels.hip', 'gru.hip', 'step.hip', 'inference.hip', 'collate_device.hip', 'capi.hip', 'profiler.hip', 'rng.hip', 'collate.cpp']
+SOURCES = ['gemm.hip', 'fused_layer.hip', 'graph_kernels.hip', 'head_kernels.hip', 'gru.hip', 'step.hip', 'inference.hip', 'norm.hip', 'conv.hip', 'scan.hip', 'collate_device.hip', 'capi.hip', 'profiler.hip', 'rng.hip', 'collate.cpp']
 # No packed fp32 instructions (v_pk_add/mul/fma_f32, which hipcc forms from ordinary float code): some of their forms have
 # given wrong results now and then on these GPUs.  The host pass of hipcc does not know the feature and says so.
 DEVICE_FLAGS = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
-HEADERS = ['psvae_internal.h', 'fused_device.h', os.path.join('..', '..', 'include', 'psvae.h')]
+HEADERS = ['psvae_internal.h', 'fused_device.h', 'seq_device.h', os.path.join('..', '..', 'include', 'psvae.h')]
 
 
 def _stale():

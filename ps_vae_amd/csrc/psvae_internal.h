@@ -35,6 +35,7 @@ enum Option {
     OPT_GRU_MULTI_CU,    // 0 / 1: single-CU / multi-CU recurrence
     OPT_GRU_TILES,       // 1 / 2 / 4 sequence tiles per workgroup of the multi-CU recurrence
     OPT_GRU_SPIN_TICKS,  // bound of a multi-CU recurrence wait in 10 ns ticks; 0: give up at once (tests the redo)
+    OPT_SCAN_CHUNKS,     // pieces of the time axis of the selective scan
     OPT_COUNT
 };
 int opt(int which);
@@ -42,7 +43,8 @@ int opt(int which);
 // ---------------------------------------------------------------- launch timer (profiler.hip)
 enum KernelClass {
     KC_GEMM_FWD = 0, KC_GEMM_DX, KC_GEMM_DW, KC_GEMM_REDUCE, KC_AGG_FWD, KC_AGG_BWD, KC_ETAB, KC_EMBED, KC_TABLE_GRAD,
-    KC_POOL, KC_PAIR_GATHER, KC_PAIR_SCATTER, KC_GRU_FWD, KC_GRU_BWD, KC_CE, KC_HEAD, KC_ADAM, KC_GINE_LAYER, KC_SCORER, KC_GINE_LAYER_BWD, KC_COUNT
+    KC_POOL, KC_PAIR_GATHER, KC_PAIR_SCATTER, KC_GRU_FWD, KC_GRU_BWD, KC_CE, KC_HEAD, KC_ADAM, KC_GINE_LAYER, KC_SCORER, KC_GINE_LAYER_BWD,
+    KC_NORM, KC_SEQ_CONV, KC_SCAN_FWD, KC_SCAN_BWD, KC_COUNT
 };
 struct ProfScope {
     ProfScope(hipStream_t s, int kc, double work);

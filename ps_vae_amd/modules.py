@@ -6,6 +6,8 @@ follow `src/modules/common_nn.py`, `encoder.py`, `predictor.py` and
 `nn.Embedding`) are used only as parameter containers so that the state-dict
 layout is the reference's; their `forward` is never called.
 """
+import math
+
 import torch
 import torch.nn as nn
 
@@ -101,6 +103,86 @@ class Encoder(nn.Module):
         if return_x:
             return res, x
         return res
+
+
+class LayerNorm(nn.LayerNorm):
+    """`nn.LayerNorm` over the last dimension, on the HIP kernel (fp32, bf16 or fp16 inputs, fp32 parameters)."""
+
+    def __init__(self, dim, eps=1e-5, elementwise_affine=True, bias=True):
+        super().__init__(dim, eps=eps, elementwise_affine=elementwise_affine, bias=bias)
+        if len(self.normalized_shape) != 1:
+            raise ValueError('the HIP kernel normalises over one dimension, the last')
+
+    def forward(self, x):
+        if x.shape[-1] != self.normalized_shape[0]:
+            raise ValueError(f'LayerNorm: the last dimension is {x.shape[-1]}, expected {self.normalized_shape[0]}')
+        return ops.layer_norm(x, self.weight, self.bias, self.eps)
+
+
+class SSMBlock(nn.Module):
+    """A pre-norm state-space block over sequences, the recurrent layer for long sequences beside the decoder's GRU (no
+    counterpart in the reference):
+
+        u, z = in_proj(norm(x));  v = silu(causal_conv(u));  r, B, C = x_proj(v)
+        out = x + out_proj(selective_scan(v, dt_proj(r), -exp(A_log), B, C, D, gate z))
+
+    `forward` takes [S, L, dim], or packed rows [T, dim] with `seq_off` (int32 [S+1]); `step` one row for each of S
+    sequences, with a state from `init_state` or from `forward(.., return_state=True)`.  fp32, as the Linear kernels."""
+
+    def __init__(self, dim, dim_inner=None, num_states=16, num_taps=4, dt_rank=None, num_groups=1):
+        super().__init__()
+        inner = 2 * dim if dim_inner is None else dim_inner
+        if inner % num_groups:
+            raise ValueError(f'{num_groups} groups do not divide {inner} channels')
+        if not 1 <= num_states <= 64 or not 1 <= num_taps <= 8:
+            raise ValueError('the HIP kernels take 1 to 64 states and 1 to 8 taps')
+        self.inner, self.num_states, self.num_groups = inner, num_states, num_groups
+        self.dt_rank = max(1, dim // 16) if dt_rank is None else dt_rank
+        self.norm = LayerNorm(dim)
+        self.in_proj = nn.Linear(dim, 2 * inner, bias=False)
+        self.conv_weight = nn.Parameter((torch.rand(inner, num_taps) * 2 - 1) / num_taps ** 0.5)
+        self.conv_bias = nn.Parameter(torch.zeros(inner))
+        self.x_proj = nn.Linear(inner, self.dt_rank + 2 * num_groups * num_states, bias=False)
+        self.dt_proj = nn.Linear(self.dt_rank, inner)      # its bias is the scan's dt_bias
+        self.A_log = nn.Parameter(torch.log(torch.arange(1, num_states + 1).float()).repeat(inner, 1))
+        self.D = nn.Parameter(torch.ones(inner))
+        self.out_proj = nn.Linear(inner, dim, bias=False)
+        with torch.no_grad():                              # steps between 1e-3 and 1e-1, through the inverse of softplus
+            step = torch.exp(torch.rand(inner) * (math.log(0.1) - math.log(0.001)) + math.log(0.001))
+            self.dt_proj.bias.copy_(step + torch.log(-torch.expm1(-step)))
+
+    def init_state(self, num_sequences):
+        """(inputs in front of the convolution, states) of sequences that have not begun."""
+        w = self.conv_weight
+        return (w.new_zeros(num_sequences, w.shape[1] - 1, self.inner), w.new_zeros(num_sequences, self.inner, self.num_states))
+
+    def _split(self, v):
+        """Steps, B and C from the convolved rows."""
+        gn = self.num_groups * self.num_states
+        p = ops.linear(v, self.x_proj.weight)
+        shape = (*v.shape[:-1], self.num_groups, self.num_states)
+        B, C = (p[..., self.dt_rank + i * gn:self.dt_rank + (i + 1) * gn].unflatten(-1, shape[-2:]) for i in range(2))
+        return ops.linear(p[..., :self.dt_rank], self.dt_proj.weight), B, C
+
+    def forward(self, x, seq_off=None, state=None, return_state=False):
+        window, h0 = (None, None) if state is None else state
+        u, z = ops.linear(self.norm(x), self.in_proj.weight).chunk(2, dim=-1)
+        v, window = ops.causal_conv(u, self.conv_weight, self.conv_bias, silu=True, seq_off=seq_off, state=window, return_state=True)
+        dt, B, C = self._split(v)
+        y, h = ops.selective_scan(v, dt, -torch.exp(self.A_log), B, C, D=self.D, z=z, dt_bias=self.dt_proj.bias, h0=h0, seq_off=seq_off,
+                                  return_state=True)
+        out = x + ops.linear(y, self.out_proj.weight)
+        return (out, (window, h)) if return_state else out
+
+    @torch.no_grad()
+    def step(self, x, state):
+        """x [S, dim]; `state` is moved on in place.  Returns the block's output rows."""
+        window, h = state
+        u, z = ops.linear(self.norm(x), self.in_proj.weight).chunk(2, dim=-1)
+        v, _ = ops.causal_conv_step(u, window, self.conv_weight, self.conv_bias, silu=True)
+        dt, B, C = self._split(v)
+        y, _ = ops.selective_scan_step(v, dt, -torch.exp(self.A_log), B, C, h, D=self.D, z=z, dt_bias=self.dt_proj.bias)
+        return x + ops.linear(y, self.out_proj.weight)
 
 
 class Predictor(nn.Module):

@@ -149,3 +149,367 @@ class SegmentPoolFn(torch.autograd.Function):
                                                    _stream()),
                    'psvae_gine_aggregate_backward(pool broadcast)')
         return dx, None, None
+
+
+# ---- sequence-block operators: layer norm, short causal convolution, selective scan -----------------------------
+# Activations are fp32, bf16 or fp16 (one type a call), [.., width]; rows may be strided views (a slice of a wider
+# projection) and are copied only where their last dimension is not contiguous.  Parameters and states are fp32.
+# Sequences are either the first dimension of a [S, L, width] tensor or, with `seq_off` (int32 [S+1] on the same device,
+# non-decreasing), rows seq_off[s] .. seq_off[s+1]-1 of a packed [T, width] tensor; without it [T, width] is one
+# sequence.  Packed rows that no sequence holds give zeros and get zero gradients.
+
+_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _run(what, device, fn, *args):
+    """The library call on the device's current stream, with that device current."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        _lib.check(rc, what)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows(t, width):
+    """`t` as rows of `width` contiguous elements and the distance of two rows; a copy only where no view does it."""
+    if t.is_contiguous():
+        return t, width
+    t = t.reshape(-1, width)
+    if (width > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < width):
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else width)
+
+
+def _act(what, name, t, like, shape):
+    """Checks an activation operand against the call's first one."""
+    if t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f'{what}: {name} is {t.dtype} on {t.device}, x is {like.dtype} on {like.device}')
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f'{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}')
+
+
+def _par(what, name, t, like, shape):
+    """A parameter or state: checked, fp32, contiguous."""
+    if t is None:
+        return None
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f'{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}')
+    if t.device != like.device:
+        raise ValueError(f'{what}: {name} is on {t.device}, x is on {like.device}')
+    if not t.is_floating_point():
+        raise ValueError(f'{what}: {name} is {t.dtype}, expected a floating type')
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
+
+
+def _first(what, x, dims):
+    _need_gpu(x, what)
+    if x.dtype not in _DTYPES:
+        raise ValueError(f'{what}: x is {x.dtype}; float32, bfloat16 and float16 are supported')
+    if x.dim() not in dims:
+        raise ValueError(f'{what}: x has {x.dim()} dimensions')
+    if x.shape[-1] < 1:
+        raise ValueError(f'{what}: x has no channels')
+
+
+def _sequences(what, x, seq_off):
+    """(rows, sequences) of x."""
+    rows = x.shape[0] if x.dim() == 2 else x.shape[0] * x.shape[1]
+    if seq_off is None:
+        return rows, (1 if x.dim() == 2 else x.shape[0])
+    if x.dim() != 2:
+        raise ValueError(f'{what}: seq_off goes with packed rows [T, width], x has {x.dim()} dimensions')
+    if seq_off.dtype != torch.int32 or seq_off.dim() != 1 or seq_off.numel() < 1 or not seq_off.is_contiguous() or seq_off.device != x.device:
+        raise ValueError(f'{what}: seq_off must be a contiguous int32 vector of sequences + 1 offsets on {x.device}')
+    if seq_off.numel() == 1 and rows:
+        raise ValueError(f'{what}: seq_off names no sequence for {rows} rows')
+    return rows, seq_off.numel() - 1
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _norm_forward(x, w, b, eps, keep):
+    H = x.shape[-1]
+    rows = x.numel() // H
+    x2, ldx = _rows(x, H)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if keep else None
+    at = stats.data_ptr() if keep else None
+    _run('psvae_layer_norm_forward', x.device, _lib.lib().psvae_layer_norm_forward, x2.data_ptr(), ldx, _ptr(w), _ptr(b), y.data_ptr(), H,
+         at, at + 4 * rows if keep else None, rows, H, eps, _DTYPES[x.dtype])
+    return y, x2, ldx, stats
+
+
+class LayerNormFn(torch.autograd.Function):
+    """y = (x - mean) / sqrt(var + eps) * w + b over the last dimension."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, eps):
+        y, x2, ctx.ldx, stats = _norm_forward(x, w, b, eps, True)
+        ctx.save_for_backward(x2, w, stats)
+        ctx.has_bias, ctx.shape = b is not None, x.shape
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        L = _lib.lib()
+        x2, w, stats = ctx.saved_tensors
+        H, rows = ctx.shape[-1], stats.shape[1]
+        need_x, need_w, need_b = ctx.needs_input_grad[0], w is not None and ctx.needs_input_grad[1], ctx.has_bias and ctx.needs_input_grad[2]
+        dy2, lddy = _rows(dy, H)
+        dev = dy.device
+        dx = torch.empty(ctx.shape, dtype=x2.dtype, device=dev) if need_x else None
+        dw = torch.empty(H, dtype=torch.float32, device=dev) if need_w else None
+        db = torch.empty(H, dtype=torch.float32, device=dev) if need_b else None
+        sc = _scratch(L.psvae_layer_norm_scratch_bytes(rows, H), dev) if need_w or need_b else None
+        _run('psvae_layer_norm_backward', dev, L.psvae_layer_norm_backward, dy2.data_ptr(), lddy, x2.data_ptr(), ctx.ldx, _ptr(w), stats.data_ptr(),
+             stats.data_ptr() + 4 * rows, _ptr(dx), H, _ptr(dw), _ptr(db), rows, H, _DTYPES[x2.dtype], _ptr(sc), sc.numel() if sc is not None else 0)
+        return dx, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """Layer norm over the last dimension of x [.., H]; weight and bias [H], each optional."""
+    _first('layer_norm', x, range(1, 65))
+    H = x.shape[-1]
+    weight, bias = _par('layer_norm', 'weight', weight, x, (H,)), _par('layer_norm', 'bias', bias, x, (H,))
+    if _wants_grad(x, weight, bias):
+        return LayerNormFn.apply(x, weight, bias, float(eps))
+    return _norm_forward(x, weight, bias, float(eps), False)[0]
+
+
+def _conv_forward(x, w, b, state, seq_off, flags, rows, S, want_state):
+    D, W = w.shape
+    x2, ldx = _rows(x, D)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = torch.empty(S, W - 1, D, dtype=x.dtype, device=x.device) if want_state else None
+    _run('psvae_causal_conv_forward', x.device, _lib.lib().psvae_causal_conv_forward, x2.data_ptr(), ldx, w.data_ptr(), _ptr(b), y.data_ptr(), D,
+         _ptr(seq_off), _ptr(state), _ptr(out), rows, S, D, W, _DTYPES[x.dtype], flags)
+    return y, out, x2, ldx
+
+
+class CausalConvFn(torch.autograd.Function):
+    """y[t] = act(b + sum_k w[:, k] x[t - W + 1 + k]) inside every sequence; returns (y, final state or None)."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, state, seq_off, flags, rows, S, want_state):
+        y, out, x2, ctx.ldx = _conv_forward(x, w, b, state, seq_off, flags, rows, S, want_state)
+        ctx.save_for_backward(x2, w, b, state, seq_off)
+        ctx.flags, ctx.rows, ctx.S, ctx.shape = flags, rows, S, x.shape
+        if out is not None:
+            ctx.mark_non_differentiable(out)
+        return y, out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, _):
+        L = _lib.lib()
+        x2, w, b, state, seq_off = ctx.saved_tensors
+        D, W = w.shape
+        dev = dy.device
+        need_x, need_w, need_b = ctx.needs_input_grad[0], ctx.needs_input_grad[1], b is not None and ctx.needs_input_grad[2]
+        dy2, lddy = _rows(dy, D)
+        dx = torch.empty(ctx.shape, dtype=x2.dtype, device=dev) if need_x else None
+        dw = torch.empty(D, W, dtype=torch.float32, device=dev) if need_w else None
+        db = torch.empty(D, dtype=torch.float32, device=dev) if need_b else None
+        dtype = _DTYPES[x2.dtype]
+        sc = _scratch(L.psvae_causal_conv_scratch_bytes(ctx.rows, D, W, dtype), dev) if need_w or need_b else None
+        _run('psvae_causal_conv_backward', dev, L.psvae_causal_conv_backward, dy2.data_ptr(), lddy, x2.data_ptr(), ctx.ldx, w.data_ptr(), _ptr(b),
+             _ptr(dx), D, _ptr(dw), _ptr(db), _ptr(seq_off), _ptr(state), ctx.rows, ctx.S, D, W, dtype, ctx.flags, _ptr(sc),
+             sc.numel() if sc is not None else 0)
+        return dx, dw, db, None, None, None, None, None, None
+
+
+def _conv_params(what, x, weight, bias):
+    if weight.dim() != 2 or not 1 <= weight.shape[1] <= 8:
+        raise ValueError(f'{what}: weight has shape {tuple(weight.shape)}, expected [channels, taps] with 1 to 8 taps')
+    D = x.shape[-1]
+    return _par(what, 'weight', weight, x, (D, weight.shape[1])), _par(what, 'bias', bias, x, (D,))
+
+
+def causal_conv(x, weight, bias=None, *, silu=False, seq_off=None, state=None, return_state=False):
+    """Short causal convolution along every sequence, one filter a channel: weight [D, W] with 1 to 8 taps (the last one
+    on the row itself), bias [D].  `state` [S, W-1, D] in x's type holds the inputs in front of every sequence (oldest
+    first; zeros without it) and carries no gradient; with `return_state` the call gives (y, state behind the end)."""
+    what = 'causal_conv'
+    _first(what, x, (2, 3))
+    rows, S = _sequences(what, x, seq_off)
+    weight, bias = _conv_params(what, x, weight, bias)
+    if state is not None:
+        _act(what, 'state', state, x, (S, weight.shape[1] - 1, x.shape[-1]))
+        if state.requires_grad:
+            raise ValueError(f'{what}: no gradient is computed for the state; pass state.detach()')
+        state = state.contiguous()
+    flags = (_lib.SEQ_SILU if silu else 0) | (_lib.SEQ_ZERO_OUTSIDE if seq_off is not None else 0)
+    if _wants_grad(x, weight, bias):
+        y, out = CausalConvFn.apply(x, weight, bias, state, seq_off, flags, rows, S, bool(return_state))
+    else:
+        y, out = _conv_forward(x, weight, bias, state, seq_off, flags, rows, S, return_state)[:2]
+    return (y, out) if return_state else y
+
+
+def causal_conv_step(x, state, weight, bias=None, *, silu=False, state_out=None):
+    """One row x [S, D] for each of S sequences.  `state` [S, W-1, D] is moved on by the row, in place or into
+    `state_out`; returns (y, the new state).  No gradients."""
+    what = 'causal_conv_step'
+    _first(what, x, (2,))
+    S, D = x.shape
+    weight, bias = _conv_params(what, x, weight, bias)
+    if _wants_grad(x, state, weight, bias):
+        raise RuntimeError(f'{what} has no backward pass: call it under torch.no_grad() or on detached tensors')
+    _act(what, 'state', state, x, (S, weight.shape[1] - 1, D))
+    out = _state_out(what, state, state_out)
+    x2, ldx = _rows(x, D)
+    y = torch.empty(S, D, dtype=x.dtype, device=x.device)
+    _run('psvae_causal_conv_step', x.device, _lib.lib().psvae_causal_conv_step, x2.data_ptr(), ldx, state.data_ptr(), out.data_ptr(), weight.data_ptr(),
+         _ptr(bias), y.data_ptr(), D, S, D, weight.shape[1], _DTYPES[x.dtype], _lib.SEQ_SILU if silu else 0)
+    return y, out
+
+
+def _state_out(what, state, out):
+    """Where a step writes its state: `out`, or `state` itself; other memory must not overlap it."""
+    if not state.is_contiguous():
+        raise ValueError(f'{what}: state must be contiguous')
+    if out is None:
+        return state
+    if out.shape != state.shape or out.dtype != state.dtype or out.device != state.device or not out.is_contiguous():
+        raise ValueError(f'{what}: state_out must be contiguous and have the shape, type and device of state')
+    a, b, n = state.data_ptr(), out.data_ptr(), state.numel() * state.element_size()
+    if a != b and a < b + n and b < a + n:
+        raise ValueError(f'{what}: state_out overlaps state without being it')
+    return out
+
+
+def _scan_struct(x, ldx, dt, lddt, A, B, ldb, C, ldc, D, z, ldz, bias, h0, seq_off, rows, S, G, flags):
+    width, N = A.shape
+    return _lib.Scan(_ptr(x), _ptr(dt), _ptr(B), _ptr(C), _ptr(z), ldx, lddt, ldb, ldc, ldz, _ptr(A), _ptr(D), _ptr(bias), _ptr(h0), _ptr(seq_off),
+                     rows, S, width, G, N, _DTYPES[x.dtype], flags)
+
+
+def _scan_rows(x, dt, B, C, z, width, G, N):
+    """The activation operands as rows, with their distances, in psvae_scan's order: x, dt, (A), B, C, (skip), z."""
+    return [_rows(x, width), _rows(dt, width), _rows(B, G * N), _rows(C, G * N), (None, 0) if z is None else _rows(z, width)]
+
+
+def _scan_forward(x, dt, A, B, C, D, z, bias, h0, seq_off, flags, rows, S, G, want_state, keep):
+    L = _lib.lib()
+    (width, N), dev = A.shape, x.device
+    ops2 = _scan_rows(x, dt, B, C, z, width, G, N)
+    (x2, ldx), (dt2, lddt), (B2, ldb), (C2, ldc), (z2, ldz) = ops2
+    a = _scan_struct(x2, ldx, dt2, lddt, A, B2, ldb, C2, ldc, D, z2, ldz, bias, h0, seq_off, rows, S, G, flags)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    last = torch.empty(S, width, N, dtype=torch.float32, device=dev) if want_state else None
+    kept = _scratch(L.psvae_selective_scan_saved_bytes(rows, S, width, G, N), dev) if keep else None
+    nbytes = L.psvae_selective_scan_scratch_bytes(rows, S, width, G, N, 0)
+    sc = _scratch(nbytes, dev) if nbytes else None
+    _run('psvae_selective_scan_forward', dev, L.psvae_selective_scan_forward, a, y.data_ptr(), width, _ptr(last), _ptr(kept), _ptr(sc), nbytes)
+    return y, last, kept, ops2
+
+
+class SelectiveScanFn(torch.autograd.Function):
+    """h[t] = exp(delta A) h[t-1] + delta x B, y = (C h + D x) silu(z) along every sequence; returns (y, last h or None)."""
+
+    @staticmethod
+    def forward(ctx, x, dt, A, B, C, D, z, bias, h0, seq_off, flags, rows, S, G, want_state):
+        y, last, kept, ops2 = _scan_forward(x, dt, A, B, C, D, z, bias, h0, seq_off, flags, rows, S, G, want_state, True)
+        (x2, _), (dt2, _), (B2, _), (C2, _), (z2, _) = ops2
+        ctx.save_for_backward(x2, dt2, A, B2, C2, D, z2, bias, seq_off, kept)
+        ctx.ld = [ld for _, ld in ops2]
+        ctx.call = flags, rows, S, G
+        ctx.shapes = x.shape, B.shape, C.shape, None if h0 is None else h0.shape
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dlast):
+        L = _lib.lib()
+        x, dt, A, B, C, D, z, bias, seq_off, kept = ctx.saved_tensors
+        flags, rows, S, G = ctx.call
+        xs, bs, cs, hs = ctx.shapes
+        ldx, lddt, ldb, ldc, ldz = ctx.ld
+        (width, N), dev = A.shape, x.device
+        dy = torch.zeros(xs, dtype=x.dtype, device=dev) if dy is None else dy
+        dy2, lddy = _rows(dy, width)
+        dlast = None if dlast is None else _f32c(dlast)
+        a = _scan_struct(x, ldx, dt, lddt, A, B, ldb, C, ldc, D, z, ldz, bias, None, seq_off, rows, S, G, flags)
+
+        def like(shape, dtype=x.dtype):
+            return torch.empty(shape, dtype=dtype, device=dev)
+        f32 = torch.float32
+        dx, ddt, dB, dC, dz = like(xs), like(xs), like(bs), like(cs), None if z is None else like(xs)
+        dA, dD = like((width, N), f32), None if D is None else like(width, f32)
+        dbias, dh0 = None if bias is None else like(width, f32), None if hs is None else like(hs, f32)
+        g = _lib.ScanGrads(_ptr(dx), _ptr(ddt), _ptr(dB), _ptr(dC), _ptr(dz), width, width, G * N, G * N, width, _ptr(dA), _ptr(dD), _ptr(dbias),
+                           _ptr(dh0))
+        nbytes = L.psvae_selective_scan_scratch_bytes(rows, S, width, G, N, 1)
+        sc = _scratch(nbytes, dev)
+        _run('psvae_selective_scan_backward', dev, L.psvae_selective_scan_backward, a, _ptr(kept), dy2.data_ptr(), lddy, _ptr(dlast), g, sc.data_ptr(),
+             sc.numel())
+        return dx, ddt, dA, dB, dC, dD, dz, dbias, dh0, None, None, None, None, None, None
+
+
+def _scan_operands(what, x, dt, A, B, C, D, z, dt_bias, h0, S):
+    """Checks; returns (A, D, dt_bias, h0) in fp32 and the number of groups."""
+    width = x.shape[-1]
+    if A.dim() != 2 or A.shape[0] != width or not 1 <= A.shape[1] <= 64:
+        raise ValueError(f'{what}: A has shape {tuple(A.shape)}, expected [{width}, states] with 1 to 64 states')
+    N, lead = A.shape[1], x.shape[:-1]
+    G = 1 if B.dim() == x.dim() else B.shape[-2] if B.dim() == x.dim() + 1 else 0
+    if G < 1 or width % G:
+        raise ValueError(f'{what}: B has shape {tuple(B.shape)}: [.., states] or [.., groups, states] with groups that divide {width}')
+    _act(what, 'dt', dt, x, x.shape)
+    _act(what, 'B', B, x, (*lead, N) if B.dim() == x.dim() else (*lead, G, N))
+    _act(what, 'C', C, x, B.shape)
+    if z is not None:
+        _act(what, 'z', z, x, x.shape)
+    return (_par(what, 'A', A, x, (width, N)), _par(what, 'D', D, x, (width,)), _par(what, 'dt_bias', dt_bias, x, (width,)),
+            _par(what, 'h0', h0, x, (S, width, N)), G)
+
+
+def selective_scan(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, softplus=True, h0=None, seq_off=None, return_state=False):
+    """Selective state space scan along every sequence:
+
+        delta = softplus(dt + dt_bias)                                      (softplus=False: dt + dt_bias)
+        h[t, d, n] = exp(delta[t, d] A[d, n]) h[t-1, d, n] + delta[t, d] x[t, d] B[t, g, n]
+        y[t, d] = (sum_n C[t, g, n] h[t, d, n] + D[d] x[t, d]) * silu(z[t, d])
+
+    x, dt, z [.., width]; B, C [.., N] or [.., G, N], each group shared by width / G neighbouring channels; A [width, N]
+    with up to 64 states; D, dt_bias [width]; h0 [S, width, N], the state in front of every sequence (zeros without
+    it).  Returns y, with `return_state` (y, the state behind every sequence's end), which carries gradients."""
+    what = 'selective_scan'
+    _first(what, x, (2, 3))
+    rows, S = _sequences(what, x, seq_off)
+    A, D, dt_bias, h0, G = _scan_operands(what, x, dt, A, B, C, D, z, dt_bias, h0, S)
+    flags = (_lib.SEQ_SOFTPLUS if softplus else 0) | (_lib.SEQ_ZERO_OUTSIDE if seq_off is not None else 0)
+    if _wants_grad(x, dt, A, B, C, D, z, dt_bias, h0):
+        y, last = SelectiveScanFn.apply(x, dt, A, B, C, D, z, dt_bias, h0, seq_off, flags, rows, S, G, bool(return_state))
+    else:
+        y, last = _scan_forward(x, dt, A, B, C, D, z, dt_bias, h0, seq_off, flags, rows, S, G, return_state, False)[:2]
+    return (y, last) if return_state else y
+
+
+def selective_scan_step(x, dt, A, B, C, state, *, D=None, z=None, dt_bias=None, softplus=True, state_out=None):
+    """One row of the scan for each of S sequences: x, dt, z [S, width], B, C [S, N] or [S, G, N].  `state` [S, width, N]
+    fp32 is moved on, in place or into `state_out`; returns (y, the new state).  No gradients."""
+    what = 'selective_scan_step'
+    _first(what, x, (2,))
+    S, width = x.shape
+    if state.dtype != torch.float32:
+        raise ValueError(f'{what}: state is {state.dtype}, expected torch.float32')
+    if _wants_grad(x, dt, A, B, C, state, D, z, dt_bias):
+        raise RuntimeError(f'{what} has no backward pass: call it under torch.no_grad() or on detached tensors')
+    out = _state_out(what, state, state_out)
+    A, D, dt_bias, state, G = _scan_operands(what, x, dt, A, B, C, D, z, dt_bias, state, S)
+    (x2, ldx), (dt2, lddt), (B2, ldb), (C2, ldc), (z2, ldz) = _scan_rows(x, dt, B, C, z, width, G, A.shape[1])
+    a = _scan_struct(x2, ldx, dt2, lddt, A, B2, ldb, C2, ldc, D, z2, ldz, dt_bias, state, None, S, S, G, _lib.SEQ_SOFTPLUS if softplus else 0)
+    y = torch.empty(S, width, dtype=x.dtype, device=x.device)
+    _run('psvae_selective_scan_step', x.device, _lib.lib().psvae_selective_scan_step, a, y.data_ptr(), width, out.data_ptr())
+    return y, out
