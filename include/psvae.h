@@ -498,7 +498,7 @@ int psvae_causal_conv_step(const void* x, int64_t ldx, const void* state, void* 
  *   h[t, d, n] = exp(delta[t, d] A[d, n]) h[t-1, d, n] + delta[t, d] x[t, d] B[t, g, n]
  *   y[t, d] = (sum_n C[t, g, n] h[t, d, n] + skip[d] x[t, d]) * silu(z[t, d])
  * x, dt, z [T, D], B and C [T, G N] of `dtype`; A [D, N], skip [D], dt_bias [D] and the states h0, hT [S, D, N] fp32,
- * contiguous.  z, skip, dt_bias, h0 (and, as outputs, hT) may be NULL.
+ * contiguous; leading dimensions below 2^26.  z, skip, dt_bias, h0 (and, as outputs, hT) may be NULL.
  * _forward: with `saved` (psvae_selective_scan_saved_bytes, 16-byte aligned; the state every 16 rows) a backward pass can
  *   follow.  scratch: psvae_selective_scan_scratch_bytes(.., backward = 0), 0 where the time axis is not cut.
  * _backward: given dy (gradient of y) and dhT (of hT, or NULL), writes every gradient of psvae_scan_grads; dz may be NULL
@@ -514,8 +514,7 @@ typedef struct psvae_scan {
     int32_t S, D, G, N, dtype, flags;
 } psvae_scan;
 typedef struct psvae_scan_grads {
-    void *dx, *ddt, *dB, *dC, *dz;
-    int64_t lddx, ldddt, lddb, lddc, lddz;
+    void *dx, *ddt, *dB, *dC, *dz;      /* contiguous, of `dtype` */
     float *dA, *d_skip, *d_dt_bias, *dh0;
 } psvae_scan_grads;
 size_t psvae_selective_scan_scratch_bytes(int64_t T, int S, int D, int G, int N, int backward);

@@ -99,7 +99,7 @@ class Scan(C.Structure):
 
 
 class ScanGrads(C.Structure):
-    _fields_ = ([(k, vp) for k in ('dx', 'ddt', 'dB', 'dC', 'dz')] + [(k, i64) for k in ('lddx', 'ldddt', 'lddb', 'lddc', 'lddz')] +
+    _fields_ = ([(k, vp) for k in ('dx', 'ddt', 'dB', 'dC', 'dz')] +
                 [(k, vp) for k in ('dA', 'd_skip', 'd_dt_bias', 'dh0')])
 
 

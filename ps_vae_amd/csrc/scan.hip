@@ -24,10 +24,11 @@
 
 namespace {
 
-constexpr int TILE = 16;         // rows a tile; also the distance of the states kept for the backward pass
+constexpr int TILE = 16;         // rows a tile
+constexpr int HALF = 8;          // rows the lanes work through at a time; the distance of the states kept for the backward pass
 constexpr int PITCH = 20;        // floats of LDS a channel's tile of rows takes: 16-byte rows that 16 channels spread over all banks
 constexpr int MAX_CHUNKS = 64;
-constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LOG2E = 1.44269504088896340736f, LOG2E_LOW = 1.92596299112661747e-8f, LN2 = 0.69314718055994530942f;
 
 // Device pointers and sizes of one call; `T` rows, `S` sequences, `D` channels in `G` groups, `N` states.
 struct Scan {
@@ -35,7 +36,7 @@ struct Scan {
     int64_t ldx, lddt, ldb, ldc, ldz, lddy;
     const float *A, *D, *bias, *h0;
     void *y, *dx, *ddt, *dz;
-    int64_t ldy, lddx, ldddt, lddz;
+    int64_t ldy;
     float *hT, *kept;
     const float* dhT;
     float* dh0;
@@ -45,11 +46,15 @@ struct Scan {
     int T, S, Dn, G, N, chunks, softplus, zero_outside, vec;
 };
 
-__device__ __forceinline__ float softplusf(float v) {
-    if (v > 20.f) return v;                // exp(-20) is below half a step of 20
-    // log(1 + e) = e log(u) / (u - 1) with u = 1 + e as rounded: the rounding of u cancels (Kahan's form, in Goldberg 1991)
-    const float e = expf(v), u = 1.f + e;
-    return u == 1.f ? e : logf(u) * (e / (u - 1.f));
+// softplus and its slope, the sigmoid, without branches.  exp(v) = 2^t (1 + r ln 2) with t = v log2 e as rounded and r what
+// the rounding (and the constant's) left out; log(1 + e) = log(u) + (e - (u - 1)) / u with u = 1 + e as rounded.  From 20
+// on exp(-v) is below half a step of v (and a NaN goes the same way); exp(-100) is zero beside anything.
+__device__ __forceinline__ float softplus_slope(float v, float& slope) {
+    const float w = __builtin_amdgcn_fmed3f(v, -100.f, 100.f), t = w * LOG2E, r = fmaf(w, LOG2E_LOW, fmaf(w, LOG2E, -t));
+    const float e0 = __builtin_amdgcn_exp2f(t), e = fmaf(e0, r * LN2, e0);
+    const float u = 1.f + e, inv = __builtin_amdgcn_rcpf(u);
+    slope = v > 20.f ? 1.f : e * inv;
+    return v <= 20.f ? fmaf(e - (u - 1.f), inv, __builtin_amdgcn_logf(u) * LN2) : v;
 }
 
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
@@ -112,27 +117,75 @@ __device__ __forceinline__ Range chunk_tiles(int len, int chunks, int c) {
     return {min(c * per, n), min((c + 1) * per, n)};
 }
 
-// Row of `kept` for tile i of a sequence that begins at row `begin`: sequences that share a row of 16 are kept apart by
-// their number, and the last index is below T / 16 + S.
-__device__ __forceinline__ int64_t kept_row(int begin, int s, int tile) { return (int64_t)(begin >> 4) + s + tile; }
+// Row of `kept` for the first half of tile i of a sequence that begins at row `begin`: sequences that share eight rows are
+// kept apart by their number, and the last index is below T / 8 + S.
+__device__ __forceinline__ int64_t kept_row(int begin, int s, int tile) { return (int64_t)(begin / HALF) + s + tile * (TILE / HALF); }
+
+// Where a channel's four rows 4 q .. lie in its PITCH floats of LDS: quarter q changes places by the channel's sixteenth, so
+// that the 16 lanes that write one row of 64 (or 32) channels reach as many bank groups.
+__device__ __forceinline__ int quarter(int q, int ch) { return 4 * (q ^ (ch >> 4 & 3)); }
+
+// V elements in the type they are stored in, so that a prefetch waits for nothing.  `base` is the same for the workgroup,
+// the lane's distance from it fits 32 bits (rows lie less than 2^26 elements apart).
+template <class T, int V> struct Raw { T v[V]; };
+template <bool VEC, class T, int V>
+__device__ __forceinline__ void fetch_row(const void* base, unsigned offset, int n, Raw<T, V>& out) {
+    asm volatile("" : "+v"(offset));       // keeps base + offset in the instruction: hoisted sums would fill the registers
+    const T* p = (const T*)((const char*)base + offset);
+    if constexpr (V == 1) {
+        out.v[0] = (T)0.f;
+        if (n > 0) out.v[0] = p[0];
+    } else {
+        typename VecOf<T, V>::type q = (T)0.f;
+        if constexpr (VEC) {
+            if (n > 0) q = *(const typename VecOf<T, V>::type*)p;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i < n) q[i] = p[i];
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) out.v[i] = q[i];
+    }
+}
+template <bool VEC, class T, int V> __device__ __forceinline__ void store_row(void* base, unsigned offset, int n, const float (&in)[V]) {
+    asm volatile("" : "+v"(offset));
+    T* p = (T*)((char*)base + offset);
+    if constexpr (VEC) {
+        if (n > 0) store_vec<V>(p, in);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < n) p[i] = (T)in[i];
+    }
+}
+// The rows of one operand as a workgroup reads or writes them: the tile's first row (uniform) and the lane's place in it.
+struct RowsOf {
+    char* base; int64_t step; unsigned offset;       // step: bytes from one tile to the next
+    __device__ __forceinline__ RowsOf(const void* p, int64_t ld, int unit, int64_t row, int col, int r, int c)
+        : base((char*)p + (row * ld + col) * unit), step(ld * unit * TILE), offset((unsigned)(r * ld + c) * unit) {}
+};
 
 // A tile's B or C, element by element (fewer than the rows' own elements by the channels over the states).
-template <class T, int P, int K>
-__device__ __forceinline__ void fetch_bc(const void* src, int64_t ld, const Scan& q, const Place& w, int row0, int rows, float (&v)[Shape<P, K>::NBC]) {
-    constexpr int NP = Shape<P, K>::NP;
+template <class T, int P, int K> struct TileBC {
+    static constexpr int NP = P * K, COUNT = Shape<P, K>::NBC;
+    T v[COUNT];
+    __device__ __forceinline__ void fetch(const char* base, int64_t ld, int N, int rows) {
 #pragma unroll
-    for (int j = 0; j < Shape<P, K>::NBC; ++j) {
-        const int e = j * 256 + threadIdx.x, r = e / NP, n = e - r * NP;
-        v[j] = r < rows && n < q.N ? (float)((const T*)src)[(int64_t)(row0 + r) * ld + w.g * q.N + n] : 0.f;
+        for (int j = 0; j < COUNT; ++j) {
+            const int e = j * 256 + threadIdx.x, r = e / NP, n = e % NP;
+            v[j] = (T)0.f;
+            unsigned at = (unsigned)(r * ld + n) * (unsigned)sizeof(T);
+            asm volatile("" : "+v"(at));
+            if (r < rows && n < N) v[j] = *(const T*)(base + at);
+        }
     }
-}
-template <int P, int K> __device__ __forceinline__ void put_bc(float* lds, const float (&v)[Shape<P, K>::NBC]) {
+    __device__ __forceinline__ void put(float* lds) const {            // lds: the workgroup's tile + threadIdx.x
 #pragma unroll
-    for (int j = 0; j < Shape<P, K>::NBC; ++j) {
-        const int e = j * 256 + threadIdx.x;
-        if (e < TILE * Shape<P, K>::NP) lds[e] = v[j];
+        for (int j = 0; j < COUNT; ++j)
+            if (j * 256 + 255 < TILE * NP || j * 256 + (int)threadIdx.x < TILE * NP) lds[j * 256] = (float)v[j];
     }
-}
+};
 
 // State of (channel d, states p K ..) in an array [rows][D][N]; lanes past the states read 0 and write nothing.
 template <int K> __device__ __forceinline__ void load_state(const float* base, int64_t row, const Scan& q, int d, int n0, float (&h)[K]) {
@@ -165,38 +218,39 @@ template <class T> __device__ __forceinline__ void zero_rows(void* out, int64_t 
 }
 
 // Forward.  ENDS: only each chunk's end state from zero and its sum of delta, for all chunks but the last.
-template <class T, int P, int K, bool ENDS>
+template <class T, int P, int K, bool VEC, bool ENDS>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(Scan q) {
     using Sh = Shape<P, K>;
-    constexpr int NP = Sh::NP, VE = Sh::VE;
-    __shared__ __attribute__((aligned(16))) float s_delta[Sh::CB * PITCH], s_dx[Sh::CB * PITCH], s_y[ENDS ? 4 : Sh::CB * PITCH];
-    __shared__ __attribute__((aligned(16))) float s_b[TILE * NP], s_c[ENDS ? 4 : TILE * NP];
+    constexpr int NP = Sh::NP, VE = Sh::VE, U = sizeof(T);
+    // LDS, one block of constant parts (so that an address is a lane's base and an immediate): delta, delta x and y of the
+    // tile by channel, B and C by row
+    constexpr int AREA = Sh::CB * PITCH, DELTA = 0, DX = AREA, BT = 2 * AREA, CT = BT + TILE * NP, YT = CT + (ENDS ? 0 : TILE * NP);
+    __shared__ __attribute__((aligned(16))) float lds[YT + (ENDS ? 0 : AREA)];
     const Place w = place<P, K>(q);
     const int chunk = blockIdx.z;
     if (!ENDS && chunk == q.chunks) { zero_rows<T>(q.y, q.ldy, q, w, gridDim.y); return; }
     const int r = threadIdx.x / Sh::TPR, c = threadIdx.x % Sh::TPR * VE;       // staging: row and first channel of this lane
     const int ch = threadIdx.x / P, n0 = threadIdx.x % P * K;                   // scanning: channel and first state
-    const int left = w.nc - c, d = w.c0 + min(ch, w.nc - 1);
-    const bool live = ch < w.nc;
+    const int left = w.nc - c, d = w.c0 + ch;
+    float *const at_row = lds + c * PITCH + quarter(r >> 2, c) + (r & 3), *const at_n = lds + n0;
+    float *const at_q[4] = {lds + ch * PITCH + quarter(0, ch), lds + ch * PITCH + quarter(1, ch), lds + ch * PITCH + quarter(2, ch),
+                            lds + ch * PITCH + quarter(3, ch)};
+    const bool live = ch < w.nc, gated = !ENDS && q.z;
     float A2[K], bias[VE], skip[VE];
-    load_state<K>(q.A, 0, q, d, n0, A2);
+    load_state<K>(live ? q.A : nullptr, 0, q, d, n0, A2);
 #pragma unroll
     for (int k = 0; k < K; ++k) A2[k] *= LOG2E;
 #pragma unroll
     for (int i = 0; i < VE; ++i) {
         bias[i] = q.bias && i < left ? q.bias[w.c0 + c + i] : 0.f;
-        skip[i] = q.D && i < left ? q.D[w.c0 + c + i] : 0.f;
+        skip[i] = !ENDS && q.D && i < left ? q.D[w.c0 + c + i] : 0.f;
     }
     for (int s = blockIdx.y; s < q.S; s += gridDim.y) {
         const SeqBounds sq = seq_bounds(q.off, s, q.S, q.T);
-        const int len = sq.end - sq.begin;
-        const Range tiles = chunk_tiles(len, q.chunks, chunk);
+        const Range tiles = chunk_tiles(sq.end - sq.begin, q.chunks, chunk);
         float h[K], sum = 0.f;
-        if (ENDS) {
-#pragma unroll
-            for (int k = 0; k < K; ++k) h[k] = 0.f;
-        } else {
-            load_state<K>(q.h0, s, q, d, n0, h);
+        load_state<K>(!ENDS && live ? q.h0 : nullptr, s, q, d, n0, h);
+        if (!ENDS && live)
             for (int i = 0; i < chunk; ++i) {          // join the chunks in front: h = exp(A sum) h + end
                 const int64_t row = (int64_t)i * q.S + s;
                 const float ds = q.chunk_s[row * q.Dn + d];
@@ -204,67 +258,80 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Scan q) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) h[k] = fmaf(__builtin_amdgcn_exp2f(ds * A2[k]), h[k], e[k]);
             }
-        }
-        float nx[VE], nt[VE], nz[VE], nb[Sh::NBC], nc[Sh::NBC];
-        auto fetch = [&](int tile) {
-            const int row0 = sq.begin + tile * TILE, rows = min(TILE, sq.end - row0), n = r < rows ? left : 0;
-            const int64_t row = row0 + min(r, rows - 1);
-            load_some<VE>((const T*)q.x + row * q.ldx + w.c0 + c, n, q.vec, nx);
-            load_some<VE>((const T*)q.dt + row * q.lddt + w.c0 + c, n, q.vec, nt);
-            if (!ENDS && q.z) load_some<VE>((const T*)q.z + row * q.ldz + w.c0 + c, n, q.vec, nz);
-            fetch_bc<T, P, K>(q.B, q.ldb, q, w, row0, rows, nb);
-            if (!ENDS) fetch_bc<T, P, K>(q.C, q.ldc, q, w, row0, rows, nc);
+        const int64_t first = sq.begin + (int64_t)tiles.first * TILE;
+        RowsOf rx(q.x, q.ldx, U, first, w.c0, r, c), rt(q.dt, q.lddt, U, first, w.c0, r, c), rz(q.z, q.ldz, U, first, w.c0, r, c),
+            ry(q.y, q.ldy, U, first, w.c0, r, c);
+        const char *pb = (const char*)q.B + (first * q.ldb + w.g * q.N) * U, *pc = (const char*)q.C + (first * q.ldc + w.g * q.N) * U;
+        float* keep = q.kept ? own_state<K>(q.kept, kept_row(sq.begin, s, tiles.first), q, NP, d, n0) : nullptr;
+        Raw<T, VE> nx, nt, nz;
+        TileBC<T, P, K> nb, nc;
+        auto fetch = [&](int rows) {
+            const int n = r < rows ? left : 0;
+            fetch_row<VEC>(rx.base, rx.offset, n, nx);
+            fetch_row<VEC>(rt.base, rt.offset, n, nt);
+            if (gated) fetch_row<VEC>(rz.base, rz.offset, n, nz);
+            nb.fetch(pb, q.ldb, q.N, rows);
+            if (!ENDS) nc.fetch(pc, q.ldc, q.N, rows);
+            rx.base += rx.step; rt.base += rt.step; rz.base += rz.step;
+            pb += q.ldb * (U * TILE); pc += q.ldc * (U * TILE);
         };
-        if (tiles.first < tiles.last) fetch(tiles.first);
-        for (int tile = tiles.first; tile < tiles.last; ++tile) {
-            const int row0 = sq.begin + tile * TILE, rows = min(TILE, sq.end - row0);
+        int remain = sq.end - (int)first;               // rows from this tile's first to the sequence's end
+        if (tiles.first < tiles.last) fetch(min(TILE, remain));
+        for (int tile = tiles.first; tile < tiles.last; ++tile, remain -= TILE) {
+            const int rows = min(TILE, remain), n = r < rows ? left : 0;
             float cx[VE], cz[VE];
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
-                const float v = nt[i] + bias[i];
-                const float delta = r < rows && i < left ? (q.softplus ? softplusf(v) : v) : 0.f;   // rows behind the end change nothing
-                cx[i] = nx[i];
-                cz[i] = nz[i];
-                s_delta[(c + i) * PITCH + r] = delta;
-                s_dx[(c + i) * PITCH + r] = delta * nx[i];
+                float v = (float)nt.v[i] + bias[i], slope;
+                if (q.softplus) v = softplus_slope(v, slope);
+                v = i < n ? v : 0.f;                     // rows behind the end change nothing
+                cx[i] = (float)nx.v[i];
+                if (gated) cz[i] = (float)nz.v[i];
+                at_row[DELTA + i * PITCH] = v;
+                at_row[DX + i * PITCH] = v * cx[i];
             }
-            put_bc<P, K>(s_b, nb);
-            if (!ENDS) put_bc<P, K>(s_c, nc);
+            nb.put(lds + BT + threadIdx.x);
+            if (!ENDS) nc.put(lds + CT + threadIdx.x);
             __syncthreads();
-            if (tile + 1 < tiles.last) fetch(tile + 1);
-            if (!ENDS && q.kept && live) put_state<K>(own_state<K>(q.kept, kept_row(sq.begin, s, tile), q, NP, d, n0), h);
+            if (tile + 1 < tiles.last) fetch(min(TILE, remain - TILE));
 #pragma unroll
-            for (int t4 = 0; t4 < TILE; t4 += 4) {
-                if (t4 < rows) {
+            for (int half = 0; half < TILE / HALF; ++half) {
+                if (half * HALF >= rows) break;
+                if (!ENDS && keep) {
+                    if (live) put_state<K>(keep, h);
+                    keep += (int64_t)q.Dn * NP;
+                }
+#pragma unroll
+                for (int t4 = half * HALF; t4 < (half + 1) * HALF; t4 += 4) {
                     float dl[4], dx[4], yv[4];
-                    lds_load<4>(s_delta + ch * PITCH + t4, dl);
-                    lds_load<4>(s_dx + ch * PITCH + t4, dx);
+                    lds_load<4>(at_q[t4 / 4] + DELTA, dl);
+                    lds_load<4>(at_q[t4 / 4] + DX, dx);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         float b[K], cc[K];
-                        lds_load<K>(s_b + (t4 + j) * NP + n0, b);
-                        if (!ENDS) lds_load<K>(s_c + (t4 + j) * NP + n0, cc);
-                        yv[j] = 0.f;
+                        lds_load<K>(at_n + BT + (t4 + j) * NP, b);
+                        if (!ENDS) lds_load<K>(at_n + CT + (t4 + j) * NP, cc);
 #pragma unroll
                         for (int k = 0; k < K; ++k) {
                             h[k] = fmaf(__builtin_amdgcn_exp2f(dl[j] * A2[k]), h[k], dx[j] * b[k]);
-                            if (!ENDS) yv[j] = fmaf(h[k], cc[k], yv[j]);
+                            if (!ENDS) yv[j] = k ? fmaf(h[k], cc[k], yv[j]) : h[k] * cc[k];
                         }
                         if (ENDS) sum += dl[j];
                         else yv[j] = lanes_add<P>(yv[j]);
                     }
-                    if (!ENDS && n0 == 0) *(float4*)(s_y + ch * PITCH + t4) = make_float4(yv[0], yv[1], yv[2], yv[3]);
+                    if (!ENDS && n0 == 0) *(float4*)(at_q[t4 / 4] + YT) = make_float4(yv[0], yv[1], yv[2], yv[3]);
                 }
             }
             __syncthreads();
-            if (!ENDS && r < rows) {
+            if (!ENDS) {
                 float o[VE];
 #pragma unroll
                 for (int i = 0; i < VE; ++i) {
-                    o[i] = fmaf(skip[i], cx[i], s_y[(c + i) * PITCH + r]);
-                    if (q.z) o[i] *= cz[i] * sigmoidf(cz[i]);
+                    o[i] = fmaf(skip[i], cx[i], at_row[YT + i * PITCH]);
+                    if (gated) o[i] *= cz[i] * sigmoidf(cz[i]);
                 }
-                store_some<VE>((T*)q.y + (int64_t)(row0 + r) * q.ldy + w.c0 + c, left, q.vec, o);
+                store_row<VEC, T, VE>(ry.base, ry.offset, n, o);
+                ry.base += ry.step;
             }
         }
         if (ENDS) {
@@ -276,51 +343,55 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Scan q) {
         } else if (q.hT && chunk == q.chunks - 1 && live) {
             save_state<K>(q.hT, s, q, d, n0, h);
         }
-        __syncthreads();                               // the last tile's s_y is read before the next sequence writes it
+        __syncthreads();                               // the last tile's y is read before the next sequence writes it
     }
 }
 
 // Backward.  CARRY: only what each chunk passes to the one in front of it, from a zero carry, and its sum of delta.
-template <class T, int P, int K, bool CARRY>
-__global__ __launch_bounds__(256) void scan_bwd_kernel(Scan q) {
+template <class T, int P, int K, bool VEC, bool CARRY>
+__global__ __launch_bounds__(256, CARRY ? 4 : 2) void scan_bwd_kernel(Scan q) {
     using Sh = Shape<P, K>;
-    constexpr int NP = Sh::NP, VE = Sh::VE;
-    // the lanes of a channel overwrite their rows of the first three with sum_n G B, sum_n G a h' A and sum_n h C
-    __shared__ __attribute__((aligned(16))) float s_delta[Sh::CB * PITCH], s_dx[CARRY ? 4 : Sh::CB * PITCH], s_dy[Sh::CB * PITCH];
-    __shared__ __attribute__((aligned(16))) float s_b[CARRY ? 4 : TILE * NP], s_c[TILE * NP];
-    __shared__ float s_bc[CARRY ? 4 : 4 * TILE * 2 * NP];
+    constexpr int NP = Sh::NP, VE = Sh::VE, U = sizeof(T);
+    // LDS, one block of constant parts: by channel what its lanes need of the rows (delta, delta x, dyp), what they make of
+    // them (sum_n G B, sum_n G a h' A2, sum_n h C) and the slope of softplus; by row B, C and the waves' sums for dB and dC
+    constexpr int AREA = Sh::CB * PITCH, DELTA = 0, DY = AREA, CT = 2 * AREA, BT = CT + TILE * NP, DX = BT + TILE * NP, SU = DX + AREA,
+                  SV = SU + AREA, SY = SV + AREA, SLOPE = SY + AREA, BC = SLOPE + AREA, BCW = TILE * 2 * NP;
+    __shared__ __attribute__((aligned(16))) float lds[CARRY ? BT : BC + 4 * BCW];
+    __shared__ float s_bias[Sh::CB], s_skip[Sh::CB];
     const Place w = place<P, K>(q);
     const int chunk = blockIdx.z + (CARRY ? 1 : 0);
     if (!CARRY && chunk == q.chunks) {
-        zero_rows<T>(q.dx, q.lddx, q, w, gridDim.y);
-        zero_rows<T>(q.ddt, q.ldddt, q, w, gridDim.y);
-        if (q.z) zero_rows<T>(q.dz, q.lddz, q, w, gridDim.y);
+        zero_rows<T>(q.dx, q.Dn, q, w, gridDim.y);
+        zero_rows<T>(q.ddt, q.Dn, q, w, gridDim.y);
+        if (q.z) zero_rows<T>(q.dz, q.Dn, q, w, gridDim.y);
         return;
     }
     const int r = threadIdx.x / Sh::TPR, c = threadIdx.x % Sh::TPR * VE;
     const int ch = threadIdx.x / P, n0 = threadIdx.x % P * K, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int left = w.nc - c, d = w.c0 + min(ch, w.nc - 1);
-    const bool live = ch < w.nc;
-    float A[K], A2[K], dA[K], bias[VE], skip[VE], dD[VE], dbias[VE];
-    load_state<K>(q.A, 0, q, d, n0, A);
+    const int left = w.nc - c, d = w.c0 + ch;
+    float *const at_row = lds + c * PITCH + quarter(r >> 2, c) + (r & 3), *const at_n = lds + n0;
+    float *const at_q[4] = {lds + ch * PITCH + quarter(0, ch), lds + ch * PITCH + quarter(1, ch), lds + ch * PITCH + quarter(2, ch),
+                            lds + ch * PITCH + quarter(3, ch)};
+    const int odd = K == 1 ? 0 : lane >> 4 & 1, copy = (lane & 15) / P;       // of the sums for dB and dC, below
+    float* const at_bc = lds + (wave * TILE * 2 + copy * 2 + (lane >> 5)) * NP + n0 + odd;
+    const bool live = ch < w.nc, gated = q.z;          // lanes without a channel compute with zeros
+    float A2[K], dA[K], dD[VE], dbias[VE];
+    load_state<K>(live ? q.A : nullptr, 0, q, d, n0, A2);
 #pragma unroll
-    for (int k = 0; k < K; ++k) { A2[k] = A[k] * LOG2E; dA[k] = 0.f; }
+    for (int k = 0; k < K; ++k) { A2[k] *= LOG2E; dA[k] = 0.f; }
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-        bias[i] = q.bias && i < left ? q.bias[w.c0 + c + i] : 0.f;
-        skip[i] = q.D && i < left ? q.D[w.c0 + c + i] : 0.f;
-        dD[i] = dbias[i] = 0.f;
+    for (int i = 0; i < VE; ++i) dD[i] = dbias[i] = 0.f;
+    for (int i = threadIdx.x; i < Sh::CB; i += 256) {
+        s_bias[i] = q.bias && i < w.nc ? q.bias[w.c0 + i] : 0.f;
+        s_skip[i] = q.D && i < w.nc ? q.D[w.c0 + i] : 0.f;
     }
+    __syncthreads();
     for (int s = blockIdx.y; s < q.S; s += gridDim.y) {
         const SeqBounds sq = seq_bounds(q.off, s, q.S, q.T);
-        const int len = sq.end - sq.begin;
-        const Range tiles = chunk_tiles(len, q.chunks, chunk);
+        const Range tiles = chunk_tiles(sq.end - sq.begin, q.chunks, chunk);
         float ag[K], sum = 0.f;                        // ag = a[t+1] G[t+1], the carry from the rows behind
-        if (CARRY) {
-#pragma unroll
-            for (int k = 0; k < K; ++k) ag[k] = 0.f;
-        } else {
-            load_state<K>(q.dhT, s, q, d, n0, ag);
+        load_state<K>(!CARRY && live ? q.dhT : nullptr, s, q, d, n0, ag);
+        if (!CARRY && live)
             for (int i = q.chunks - 1; i > chunk; --i) {
                 const int64_t row = (int64_t)(i - 1) * q.S + s;
                 const float ds = q.chunk_s[row * q.Dn + d];
@@ -328,167 +399,189 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(Scan q) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) ag[k] = fmaf(__builtin_amdgcn_exp2f(ds * A2[k]), ag[k], e[k]);
             }
-        }
-        float nx[VE], nt[VE], nz[VE], ng[VE], nb[Sh::NBC], nc[Sh::NBC], nh[K];
-        auto fetch = [&](int tile) {
-            const int row0 = sq.begin + tile * TILE, rows = min(TILE, sq.end - row0), n = r < rows ? left : 0;
-            const int64_t row = row0 + min(r, rows - 1);
-            load_some<VE>((const T*)q.dt + row * q.lddt + w.c0 + c, n, q.vec, nt);
-            load_some<VE>((const T*)q.dy + row * q.lddy + w.c0 + c, n, q.vec, ng);
-            if (q.z) load_some<VE>((const T*)q.z + row * q.ldz + w.c0 + c, n, q.vec, nz);
-            fetch_bc<T, P, K>(q.C, q.ldc, q, w, row0, rows, nc);
-            if (!CARRY) {
-                load_some<VE>((const T*)q.x + row * q.ldx + w.c0 + c, n, q.vec, nx);
-                fetch_bc<T, P, K>(q.B, q.ldb, q, w, row0, rows, nb);
-                const float* k0 = own_state<K>(q.kept, kept_row(sq.begin, s, tile), q, NP, d, n0);
+        const int64_t first = sq.begin + (int64_t)(tiles.last - 1) * TILE;     // the last tile's first row
+        RowsOf rx(q.x, q.ldx, U, first, w.c0, r, c), rt(q.dt, q.lddt, U, first, w.c0, r, c), rz(q.z, q.ldz, U, first, w.c0, r, c),
+            rg(q.dy, q.lddy, U, first, w.c0, r, c);
+        const unsigned out = (unsigned)(r * q.Dn + c) * U;
+        int64_t out0 = (first * q.Dn + w.c0) * U;      // the gradients are contiguous
+        const char *pb = (const char*)q.B + (first * q.ldb + w.g * q.N) * U, *pc = (const char*)q.C + (first * q.ldc + w.g * q.N) * U;
+        const float* keep = CARRY ? nullptr : own_state<K>(q.kept, kept_row(sq.begin, s, tiles.last - 1), q, NP, d, n0);
+        float* bc_out = CARRY ? nullptr : q.part_bc + (((int64_t)w.blk * q.T + first) * q.G + w.g) * 2 * NP;
+        Raw<T, VE> nx, nt, nz, ng;
+        TileBC<T, P, K> nb, nc;
+        float nh[TILE / HALF][K];
+        auto fetch = [&](int rows) {
+            const int n = r < rows ? left : 0;
+            fetch_row<VEC>(rt.base, rt.offset, n, nt);
+            fetch_row<VEC>(rg.base, rg.offset, n, ng);
+            if (gated) fetch_row<VEC>(rz.base, rz.offset, n, nz);
+            nc.fetch(pc, q.ldc, q.N, rows);
+            rt.base -= rt.step; rg.base -= rg.step; rz.base -= rz.step;
+            pc -= q.ldc * (U * TILE);
+            if constexpr (!CARRY) {
+                fetch_row<VEC>(rx.base, rx.offset, n, nx);
+                nb.fetch(pb, q.ldb, q.N, rows);
 #pragma unroll
-                for (int k = 0; k < K; ++k) nh[k] = k0[k];
+                for (int half = 0; half < TILE / HALF; ++half)
+#pragma unroll
+                    for (int k = 0; k < K; ++k) nh[half][k] = live && half * HALF < rows ? keep[(int64_t)half * q.Dn * NP + k] : 0.f;
+                rx.base -= rx.step;
+                pb -= q.ldb * (U * TILE);
+                keep -= (int64_t)q.Dn * NP * (TILE / HALF);
             }
         };
-        if (tiles.first < tiles.last) fetch(tiles.last - 1);
-        for (int tile = tiles.last - 1; tile >= tiles.first; --tile) {
-            const int row0 = sq.begin + tile * TILE, rows = min(TILE, sq.end - row0);
-            float cx[VE], cz[VE], cg[VE], cv[VE], cd[VE], h[K];
+        int rows = sq.end - (int)first;                 // the last tile of the sequence may be short
+        rows = min(rows, TILE);
+        if (tiles.first < tiles.last) fetch(rows);
+        for (int tile = tiles.last - 1; tile >= tiles.first; --tile, rows = TILE) {
+            const int n = r < rows ? left : 0;
+            Raw<T, VE> cx = nx, cz = nz, cg = ng;
+            float h[TILE / HALF][K];
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
-                cv[i] = nt[i] + bias[i];
-                cd[i] = r < rows && i < left ? (q.softplus ? softplusf(cv[i]) : cv[i]) : 0.f;
-                cx[i] = nx[i]; cz[i] = nz[i]; cg[i] = ng[i];
-                s_delta[(c + i) * PITCH + r] = cd[i];
-                if (!CARRY) s_dx[(c + i) * PITCH + r] = cd[i] * cx[i];
-                s_dy[(c + i) * PITCH + r] = q.z ? cg[i] * cz[i] * sigmoidf(cz[i]) : cg[i];
+                float v = (float)nt.v[i] + s_bias[c + i], dy = (float)cg.v[i], slope = 1.f;
+                if (q.softplus) v = softplus_slope(v, slope);
+                v = i < n ? v : 0.f;                     // rows behind the end change nothing
+                if (gated) dy *= (float)cz.v[i] * sigmoidf((float)cz.v[i]);
+                at_row[DELTA + i * PITCH] = v;
+                at_row[DY + i * PITCH] = dy;
+                if constexpr (!CARRY) { at_row[DX + i * PITCH] = v * (float)cx.v[i]; at_row[SLOPE + i * PITCH] = slope; }
             }
-            if (!CARRY) put_bc<P, K>(s_b, nb);
-            put_bc<P, K>(s_c, nc);
+            if constexpr (!CARRY) nb.put(lds + BT + threadIdx.x);
+            nc.put(lds + CT + threadIdx.x);
 #pragma unroll
-            for (int k = 0; k < K; ++k) h[k] = nh[k];
+            for (int half = 0; half < TILE / HALF; ++half)
+#pragma unroll
+                for (int k = 0; k < K; ++k) h[half][k] = nh[half][k];
             __syncthreads();
-            if (tile > tiles.first) fetch(tile - 1);
+            if (tile > tiles.first) fetch(TILE);
             if constexpr (CARRY) {
 #pragma unroll
-                for (int t4 = TILE - 4; t4 >= 0; t4 -= 4) {
-                    if (t4 >= rows) continue;
-                    float dl[4], dy[4];
-                    lds_load<4>(s_delta + ch * PITCH + t4, dl);
-                    lds_load<4>(s_dy + ch * PITCH + t4, dy);
+                for (int half = TILE / HALF - 1; half >= 0; --half) {
+                    if (half * HALF >= rows) continue;
 #pragma unroll
-                    for (int j = 3; j >= 0; --j) {
-                        float cc[K];
-                        lds_load<K>(s_c + (t4 + j) * NP + n0, cc);
-                        sum += dl[j];
+                    for (int t4 = (half + 1) * HALF - 4; t4 >= half * HALF; t4 -= 4) {
+                        float dl[4], dy[4];
+                        lds_load<4>(at_q[t4 / 4] + DELTA, dl);
+                        lds_load<4>(at_q[t4 / 4] + DY, dy);
 #pragma unroll
-                        for (int k = 0; k < K; ++k) ag[k] = __builtin_amdgcn_exp2f(dl[j] * A2[k]) * fmaf(dy[j], cc[k], ag[k]);
+                        for (int j = 3; j >= 0; --j) {
+                            float cc[K];
+                            lds_load<K>(at_n + CT + (t4 + j) * NP, cc);
+                            sum += dl[j];
+#pragma unroll
+                            for (int k = 0; k < K; ++k) ag[k] = __builtin_amdgcn_exp2f(dl[j] * A2[k]) * fmaf(dy[j], cc[k], ag[k]);
+                        }
                     }
                 }
                 __syncthreads();
             } else {
-            // forward over the tile: the decays a and the decayed states a h[t-1] stay in registers
-            float a[TILE][K], p[TILE][K], dAt[K];
+                float dAt[K];
 #pragma unroll
-            for (int k = 0; k < K; ++k) dAt[k] = 0.f;
+                for (int k = 0; k < K; ++k) dAt[k] = 0.f;
 #pragma unroll
-            for (int t4 = 0; t4 < TILE; t4 += 4) {
-                if (t4 >= rows) continue;
-                float dl[4], dx[4];
-                lds_load<4>(s_delta + ch * PITCH + t4, dl);
-                lds_load<4>(s_dx + ch * PITCH + t4, dx);
+                for (int half = TILE / HALF - 1; half >= 0; --half) {
+                    if (half * HALF >= rows) continue;
+                    // forward over eight rows from the kept state: the decays a and the decayed states a h[t-1] stay in registers
+                    float a[HALF][K], p[HALF][K];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float b[K];
-                    lds_load<K>(s_b + (t4 + j) * NP + n0, b);
+                    for (int t4 = 0; t4 < HALF; t4 += 4) {
+                        float dl[4], dx[4];
+                        lds_load<4>(at_q[half * 2 + t4 / 4] + DELTA, dl);
+                        lds_load<4>(at_q[half * 2 + t4 / 4] + DX, dx);
 #pragma unroll
-                    for (int k = 0; k < K; ++k) {
-                        a[t4 + j][k] = __builtin_amdgcn_exp2f(dl[j] * A2[k]);
-                        p[t4 + j][k] = a[t4 + j][k] * h[k];
-                        h[k] = fmaf(dx[j], b[k], p[t4 + j][k]);
+                        for (int j = 0; j < 4; ++j) {
+                            float b[K];
+                            lds_load<K>(at_n + BT + (half * HALF + t4 + j) * NP, b);
+#pragma unroll
+                            for (int k = 0; k < K; ++k) {
+                                a[t4 + j][k] = __builtin_amdgcn_exp2f(dl[j] * A2[k]);
+                                p[t4 + j][k] = a[t4 + j][k] * h[half][k];
+                                h[half][k] = fmaf(dx[j], b[k], p[t4 + j][k]);
+                            }
+                        }
                     }
-                }
-            }
 #pragma unroll
-            for (int t4 = TILE - 4; t4 >= 0; t4 -= 4) {
-                if (t4 >= rows) continue;
-                float dl[4], dx[4], dy[4], su[4], sv[4], sy[4];
-                lds_load<4>(s_delta + ch * PITCH + t4, dl);
-                lds_load<4>(s_dx + ch * PITCH + t4, dx);
-                lds_load<4>(s_dy + ch * PITCH + t4, dy);
+                    for (int t4 = HALF - 4; t4 >= 0; t4 -= 4) {
+                        float *const rows4 = at_q[half * 2 + t4 / 4];
+                        float dl[4], dx[4], dy[4], su[4], sv[4], sy[4], e[4][K > 1 ? K / 2 : 1];
+                        lds_load<4>(rows4 + DELTA, dl);
+                        lds_load<4>(rows4 + DX, dx);
+                        lds_load<4>(rows4 + DY, dy);
 #pragma unroll
-                for (int j = 3; j >= 0; --j) {
-                    const int t = t4 + j;
-                    float b[K], cc[K], db[K], dc[K];
-                    lds_load<K>(s_b + t * NP + n0, b);
-                    lds_load<K>(s_c + t * NP + n0, cc);
-                    su[j] = sv[j] = sy[j] = 0.f;
+                        for (int j = 3; j >= 0; --j) {
+                            const int t = half * HALF + t4 + j;
+                            float b[K], cc[K], db[K], dc[K];
+                            lds_load<K>(at_n + BT + t * NP, b);
+                            lds_load<K>(at_n + CT + t * NP, cc);
 #pragma unroll
-                    for (int k = 0; k < K; ++k) {
-                        const float g = fmaf(dy[j], cc[k], ag[k]);
-                        const float hk = fmaf(dx[j], b[k], p[t][k]);
-                        const float v = g * p[t][k];
-                        dc[k] = live ? dy[j] * hk : 0.f;
-                        db[k] = live ? g * dx[j] : 0.f;
-                        su[j] = fmaf(g, b[k], su[j]);
-                        sv[j] = fmaf(v, A[k], sv[j]);
-                        sy[j] = fmaf(hk, cc[k], sy[j]);
-                        dAt[k] = fmaf(v, dl[j], dAt[k]);
-                        ag[k] = a[t][k] * g;
-                    }
-                    su[j] = lanes_add<P>(su[j]);
-                    sv[j] = lanes_add<P>(sv[j]);
-                    sy[j] = lanes_add<P>(sy[j]);
-                    // sums over this wave's channels: row of 16 lanes 0, 1: dB of even, odd k; rows 2, 3: dC
-                    float* bc = s_bc + ((wave * TILE + t) * 2 + (lane >> 5)) * NP + n0;
-                    float f[K];
+                            for (int k = 0; k < K; ++k) {
+                                const float g = fmaf(dy[j], cc[k], ag[k]);
+                                const float hk = fmaf(dx[j], b[k], p[t4 + j][k]);
+                                const float v = g * p[t4 + j][k];
+                                dc[k] = dy[j] * hk;
+                                db[k] = g * dx[j];
+                                su[j] = k ? fmaf(g, b[k], su[j]) : g * b[k];
+                                sv[j] = k ? fmaf(v, A2[k], sv[j]) : v * A2[k];
+                                sy[j] = k ? fmaf(hk, cc[k], sy[j]) : hk * cc[k];
+                                dAt[k] = fmaf(v, dl[j], dAt[k]);
+                                ag[k] = a[t4 + j][k] * g;
+                            }
+                            su[j] = lanes_add<P>(su[j]);
+                            sv[j] = lanes_add<P>(sv[j]);
+                            sy[j] = lanes_add<P>(sy[j]);
+                            // sums over this wave's channels: rows 0, 1 of 16 lanes get dB of even, odd k; rows 2, 3 dC
+                            float f[K];
 #pragma unroll
-                    for (int k = 0; k < K; ++k) f[k] = fold32(db[k], dc[k]);
-                    const int odd = lane >> 4 & 1;
-                    if constexpr (K == 1) {
-                        const float e = stride_add<P>(f[0] + __shfl_xor(f[0], 16, 64));
-                        if ((lane & 31) < P) bc[0] = e;
-                    } else {
+                            for (int k = 0; k < K; ++k) f[k] = fold32(db[k], dc[k]);
+                            if constexpr (K == 1) e[j][0] = stride_add<P>(fold16(f[0], f[0]));
+                            else
 #pragma unroll
-                        for (int k = 0; k < K; k += 2) {
-                            const float e = stride_add<P>(fold16(f[k], f[k + 1]));
-                            if ((lane & 15) < P) bc[k + odd] = e;
+                                for (int k = 0; k < K; k += 2) e[j][k / 2] = stride_add<P>(fold16(f[k], f[k + 1]));
+                        }
+                        // the lanes of a row that hold the same states write one of the four steps each
+                        constexpr int COPIES = P < 16 ? 16 / P : 1;
+#pragma unroll
+                        for (int k = 0; k < (K > 1 ? K / 2 : 1); ++k)
+#pragma unroll
+                            for (int j0 = 0; j0 < 4; j0 += COPIES) {
+                                float v = e[j0][k];
+#pragma unroll
+                                for (int j = 1; j < COPIES; ++j) v = copy == j ? e[j0 + j][k] : v;
+                                at_bc[BC + (half * HALF + t4 + j0) * 2 * NP + 2 * k] = v;
+                            }
+                        if (n0 == 0) {
+                            *(float4*)(rows4 + SU) = make_float4(su[0], su[1], su[2], su[3]);
+                            *(float4*)(rows4 + SV) = make_float4(sv[0], sv[1], sv[2], sv[3]);
+                            *(float4*)(rows4 + SY) = make_float4(sy[0], sy[1], sy[2], sy[3]);
                         }
                     }
                 }
-                if (n0 == 0) {
-                    *(float4*)(s_delta + ch * PITCH + t4) = make_float4(su[0], su[1], su[2], su[3]);
-                    *(float4*)(s_dx + ch * PITCH + t4) = make_float4(sv[0], sv[1], sv[2], sv[3]);
-                    *(float4*)(s_dy + ch * PITCH + t4) = make_float4(sy[0], sy[1], sy[2], sy[3]);
-                }
-            }
 #pragma unroll
-            for (int k = 0; k < K; ++k) dA[k] += dAt[k];     // tile sums first: a long sum of short ones rounds less
-            __syncthreads();
-            if (r < rows) {
+                for (int k = 0; k < K; ++k) dA[k] += dAt[k];     // tile sums first: a long sum of short ones rounds less
+                __syncthreads();
                 float odx[VE], odt[VE], odz[VE];
 #pragma unroll
                 for (int i = 0; i < VE; ++i) {
-                    const int at = (c + i) * PITCH + r;
-                    const float su = s_delta[at], sv = s_dx[at], ypre = fmaf(skip[i], cx[i], s_dy[at]);
-                    float dyp = cg[i];
-                    if (q.z) {
-                        const float sg = sigmoidf(cz[i]);
-                        dyp = cg[i] * cz[i] * sg;
-                        odz[i] = cg[i] * ypre * sg * (1.f + cz[i] * (1.f - sg));
+                        const float x = (float)cx.v[i], su = at_row[SU + i * PITCH], dyp = at_row[DY + i * PITCH], skip = s_skip[c + i];
+                    if (gated) {
+                        const float z = (float)cz.v[i], sg = sigmoidf(z);
+                        odz[i] = (float)cg.v[i] * fmaf(skip, x, at_row[SY + i * PITCH]) * sg * fmaf(z, 1.f - sg, 1.f);
                     }
-                    odx[i] = fmaf(su, cd[i], skip[i] * dyp);
-                    odt[i] = fmaf(su, cx[i], sv);
-                    if (q.softplus) odt[i] *= cv[i] > 20.f ? 1.f : sigmoidf(cv[i]);
-                    dD[i] = fmaf(dyp, cx[i], dD[i]);
+                    odx[i] = fmaf(su, at_row[DELTA + i * PITCH], skip * dyp);
+                    odt[i] = i < n ? fmaf(su, x, at_row[SV + i * PITCH] * LN2) * at_row[SLOPE + i * PITCH] : 0.f;   // rows behind the end hold no sums
+                    dD[i] = fmaf(dyp, x, dD[i]);
                     dbias[i] += odt[i];
                 }
-                const int64_t row = row0 + r;
-                store_some<VE>((T*)q.dx + row * q.lddx + w.c0 + c, left, q.vec, odx);
-                store_some<VE>((T*)q.ddt + row * q.ldddt + w.c0 + c, left, q.vec, odt);
-                if (q.z) store_some<VE>((T*)q.dz + row * q.lddz + w.c0 + c, left, q.vec, odz);
-            }
-            for (int e = threadIdx.x; e < rows * 2 * NP; e += 256) {
-                const float v = (s_bc[e] + s_bc[TILE * 2 * NP + e]) + (s_bc[2 * TILE * 2 * NP + e] + s_bc[3 * TILE * 2 * NP + e]);
-                const int row = e / (2 * NP), col = e - row * 2 * NP;
-                q.part_bc[(((int64_t)w.blk * q.T + row0 + row) * q.G + w.g) * 2 * NP + col] = v;
-            }
-            __syncthreads();
+                store_row<VEC, T, VE>((char*)q.dx + out0, out, n, odx);
+                store_row<VEC, T, VE>((char*)q.ddt + out0, out, n, odt);
+                if (gated) store_row<VEC, T, VE>((char*)q.dz + out0, out, n, odz);
+                out0 -= (int64_t)q.Dn * U * TILE;
+                for (int i = threadIdx.x; i < rows * 2 * NP; i += 256)
+                    bc_out[(int64_t)(i / (2 * NP)) * q.G * 2 * NP + i % (2 * NP)] =
+                        (lds[BC + i] + lds[BC + BCW + i]) + (lds[BC + 2 * BCW + i] + lds[BC + 3 * BCW + i]);
+                bc_out -= (int64_t)q.G * 2 * NP * TILE;
+                __syncthreads();
             }
         }
         if (CARRY) {
@@ -506,12 +599,12 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(Scan q) {
         if (live) put_state<K>(own_state<K>(q.part_a, slot, q, NP, d, n0), dA);
         // dD and ddt_bias: join the 16 rows of lanes that hold the same channels
 #pragma unroll
-        for (int i = 0; i < VE; ++i) { s_delta[(c + i) * PITCH + r] = dD[i]; s_dy[(c + i) * PITCH + r] = dbias[i]; }
+        for (int i = 0; i < VE; ++i) { at_row[DELTA + i * PITCH] = dD[i]; at_row[DY + i * PITCH] = dbias[i]; }
         __syncthreads();
         for (int i = threadIdx.x; i < w.nc; i += 256) {
             float u = 0.f, v = 0.f;
 #pragma unroll
-            for (int k = 0; k < TILE; ++k) { u += s_delta[i * PITCH + k]; v += s_dy[i * PITCH + k]; }
+            for (int k = 0; k < TILE; ++k) { u += lds[DELTA + i * PITCH + k]; v += lds[DY + i * PITCH + k]; }
             q.part_d[slot * 2 * q.Dn + w.c0 + i] = u;
             q.part_d[slot * 2 * q.Dn + q.Dn + w.c0 + i] = v;
         }
@@ -522,95 +615,112 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(Scan q) {
 struct ScanJoin {
     const float *part_bc, *part_a, *part_d;
     void *dB, *dC;
-    int64_t lddb, lddc;
     float *dA, *dD, *dbias;
     const int32_t* off;
-    int T, S, Dn, G, N, NP, tiles, parts, blocks_bc, blocks_a, zero_outside;
+    int T, S, Dn, G, N, NP, tiles, parts, blocks_bc, blocks_a, zero_outside, vec;
 };
+// Sum of column `col` over `parts` rows `step` floats apart by the four quarters of the workgroup, 64 columns side by side;
+// the first quarter gets it.
+__device__ __forceinline__ float parts_sum(const float* p, int parts, int64_t step, bool inside, float (*red)[64]) {
+    const int quarter = threadIdx.x >> 6;
+    float s = 0.f;
+    if (inside)
+#pragma unroll 8
+        for (int i = quarter; i < parts; i += 4) s += p[i * step];
+    red[quarter][threadIdx.x & 63] = s;
+    __syncthreads();
+    return (red[0][threadIdx.x & 63] + red[1][threadIdx.x & 63]) + (red[2][threadIdx.x & 63] + red[3][threadIdx.x & 63]);
+}
 template <class T> __global__ __launch_bounds__(256) void scan_join_kernel(ScanJoin q) {
+    __shared__ float red[4][64];
     int blk = blockIdx.x;
-    if (blk < q.blocks_bc) {
+    if (blk < q.blocks_bc) {                            // four states of a row at a time
         const int64_t cols = (int64_t)q.T * q.G * 2 * q.NP;
         int begin = 0, end = q.T;                       // rows that a sequence holds
         if (q.off) {
             begin = min(max(q.off[0], 0), q.T);
             end = min(max(q.off[q.S], begin), q.T);
         }
-        for (int64_t i = (int64_t)blk * 256 + threadIdx.x; i < cols; i += (int64_t)q.blocks_bc * 256) {
-            const int n = (int)(i % q.NP), isC = (int)(i / q.NP & 1), g = (int)(i / (2 * q.NP) % q.G);
-            const int64_t row = i / (2 * q.NP) / q.G;
+        for (int64_t i = ((int64_t)blk * 256 + threadIdx.x) * 4; i < cols; i += (int64_t)q.blocks_bc * 1024) {
+            const int at = (int)(i % (2 * q.NP)), isC = at >= q.NP, n = at - isC * q.NP;
+            const int64_t rg = i / (2 * q.NP), row = rg / q.G;
             if (n >= q.N) continue;
-            float s = 0.f;
-            if (row >= begin && row < end)
-                for (int p = 0; p < q.tiles; ++p) s += q.part_bc[(int64_t)p * cols + i];
-            else if (!q.zero_outside) continue;
-            if (isC) ((T*)q.dC)[row * q.lddc + g * q.N + n] = (T)s;
-            else ((T*)q.dB)[row * q.lddb + g * q.N + n] = (T)s;
+            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row >= begin && row < end) {
+#pragma unroll 8
+                for (int p = 0; p < q.tiles; ++p) {
+                    const float4 v = *(const float4*)(q.part_bc + (int64_t)p * cols + i);
+                    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+                }
+            } else if (!q.zero_outside) {
+                continue;
+            }
+            const float o[4] = {s.x, s.y, s.z, s.w};
+            store_some<4>((T*)(isC ? q.dC : q.dB) + rg * q.N + n, q.N - n, q.vec, o);
         }
         return;
     }
     blk -= q.blocks_bc;
+    const int lane = threadIdx.x & 63;
     if (blk < q.blocks_a) {
-        const int64_t i = (int64_t)blk * 256 + threadIdx.x;
-        if (i >= (int64_t)q.Dn * q.N) return;
-        const int64_t at = i / q.N * q.NP + i % q.N, step = (int64_t)q.Dn * q.NP;
-        float s = 0.f;
-        for (int p = 0; p < q.parts; ++p) s += q.part_a[p * step + at];
-        q.dA[i] = s;
+        const int64_t i = (int64_t)blk * 64 + lane, all = (int64_t)q.Dn * q.N;
+        const float s = parts_sum(q.part_a + i / q.N * q.NP + i % q.N, q.parts, (int64_t)q.Dn * q.NP, i < all, red);
+        if (threadIdx.x < 64 && i < all) q.dA[i] = s;
         return;
     }
     blk -= q.blocks_a;
-    const int i = blk * 256 + threadIdx.x;
-    if (i >= q.Dn) return;
-    float u = 0.f, v = 0.f;
-    for (int p = 0; p < q.parts; ++p) {
-        u += q.part_d[(int64_t)p * 2 * q.Dn + i];
-        v += q.part_d[(int64_t)p * 2 * q.Dn + q.Dn + i];
-    }
-    if (q.dD) q.dD[i] = u;
-    if (q.dbias) q.dbias[i] = v;
+    const int i = blk * 64 + lane;                      // [2][D]: dD, then ddt_bias
+    const float s = parts_sum(q.part_d + i, q.parts, 2 * (int64_t)q.Dn, i < 2 * q.Dn, red);
+    float* out = i < q.Dn ? q.dD : q.dbias;
+    if (threadIdx.x < 64 && i < 2 * q.Dn && out) out[i < q.Dn ? i : i - q.Dn] = s;
 }
 
-// One token for each of S sequences: bound by the states, read and written once.  P lanes a channel as above; a lane has
-// its states to itself, so `hT` may be `h0`.
-template <class T, int P, int K> __global__ __launch_bounds__(256) void scan_step_kernel(Scan q, int vec_state) {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / P;
-    const int n0 = threadIdx.x % P * K;
-    if (i >= (int64_t)q.S * q.Dn) return;              // whole groups of P lanes
-    const int64_t s = i / q.Dn;
-    const int d = (int)(i - s * q.Dn), g = d / (q.Dn / q.G);
-    float h[K], A[K];
-    if (vec_state) {
-        load_vec<K>(q.h0 + i * q.N + n0, h);
-        load_vec<K>(q.A + (int64_t)d * q.N + n0, A);
-    } else {
-        load_state<K>(q.h0, s, q, d, n0, h);
-        load_state<K>(q.A, 0, q, d, n0, A);
-    }
-    const float x = (float)((const T*)q.x)[s * q.ldx + d];
-    const float v = (float)((const T*)q.dt)[s * q.lddt + d] + (q.bias ? q.bias[d] : 0.f);
-    const float delta = q.softplus ? softplusf(v) : v;
-    float y = 0.f;
+// One token for each of S sequences: bound by the states, read and written once.  P lanes a channel as above; a lane takes
+// its channel in R sequences, whose states it has all in flight at once, and has them to itself, so `hT` may be `h0`.
+template <class T, int P, int K, int R> __global__ __launch_bounds__(256) void scan_step_kernel(Scan q, int vec_state) {
+    const int wide = (q.Dn * P + 255) / 256;           // workgroups side by side over the channels
+    const int d = (blockIdx.x % wide * 256 + threadIdx.x) / P, n0 = threadIdx.x % P * K;
+    const int s0 = blockIdx.x / wide * R;
+    if (d >= q.Dn) return;                             // whole groups of P lanes
+    const int g = d / (q.Dn / q.G);
+    float h[R][K], A[K], x[R], v[R], z[R], b[R][K], c[R][K];
+    const float bias = q.bias ? q.bias[d] : 0.f, skip = q.D ? q.D[d] : 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int n = n0 + k < q.N ? n0 + k : 0;
-        const float b = (float)((const T*)q.B)[s * q.ldb + g * q.N + n], c = (float)((const T*)q.C)[s * q.ldc + g * q.N + n];
-        h[k] = fmaf(__builtin_amdgcn_exp2f(delta * (A[k] * LOG2E)), h[k], delta * x * b);
-        if (n0 + k < q.N) y = fmaf(h[k], c, y);
-    }
-    y = lanes_add<P>(y);
-    if (vec_state) {
-        store_vec<K>(q.hT + i * q.N + n0, h);
-    } else {
-        save_state<K>(q.hT, s, q, d, n0, h);
-    }
-    if (n0 == 0) {
-        if (q.D) y = fmaf(q.D[d], x, y);
-        if (q.z) {
-            const float z = (float)((const T*)q.z)[s * q.ldz + d];
-            y *= z * sigmoidf(z);
+    for (int i = 0; i < R; ++i) {
+        const int s = min(s0 + i, q.S - 1);
+        if (vec_state) load_vec<K>(q.h0 + ((int64_t)s * q.Dn + d) * q.N + n0, h[i]);
+        else load_state<K>(q.h0, s, q, d, n0, h[i]);
+        x[i] = (float)((const T*)q.x)[s * q.ldx + d];
+        v[i] = (float)((const T*)q.dt)[s * q.lddt + d] + bias;
+        z[i] = q.z ? (float)((const T*)q.z)[s * q.ldz + d] : 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int n = n0 + k < q.N ? n0 + k : 0;
+            b[i][k] = (float)((const T*)q.B)[s * q.ldb + g * q.N + n];
+            c[i][k] = n0 + k < q.N ? (float)((const T*)q.C)[s * q.ldc + g * q.N + n] : 0.f;
         }
-        ((T*)q.y)[s * q.ldy + d] = (T)y;
+    }
+    if (vec_state) load_vec<K>(q.A + (int64_t)d * q.N + n0, A);
+    else load_state<K>(q.A, 0, q, d, n0, A);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int s = s0 + i;
+        if (s >= q.S) return;
+        float delta = v[i], slope, y = 0.f;
+        if (q.softplus) delta = softplus_slope(v[i], slope);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            h[i][k] = fmaf(__builtin_amdgcn_exp2f(delta * (A[k] * LOG2E)), h[i][k], delta * x[i] * b[i][k]);
+            if (n0 + k < q.N) y = fmaf(h[i][k], c[i][k], y);
+        }
+        y = lanes_add<P>(y);
+        if (vec_state) store_vec<K>(q.hT + ((int64_t)s * q.Dn + d) * q.N + n0, h[i]);
+        else save_state<K>(q.hT, s, q, d, n0, h[i]);
+        if (n0 == 0) {
+            y = fmaf(skip, x[i], y);
+            if (q.z) y *= z[i] * sigmoidf(z[i]);
+            ((T*)q.y)[s * q.ldy + d] = (T)y;
+        }
     }
 }
 
@@ -657,6 +767,8 @@ int scan_operands(const psvae_scan* a) {
     if (a->flags & ~(PSVAE_SEQ_SOFTPLUS | PSVAE_SEQ_ZERO_OUTSIDE)) return PSVAE_E_SHAPE;
     if (a->T > 0 && (!a->x || !a->dt || !a->B || !a->C)) return PSVAE_E_NULL;
     if (!a->A) return PSVAE_E_NULL;
+    constexpr int64_t FAR = 1 << 26;       // a tile's rows lie within 32-bit distances
+    if (a->ldx >= FAR || a->lddt >= FAR || a->ldb >= FAR || a->ldc >= FAR || (a->z && a->ldz >= FAR)) return PSVAE_E_SHAPE;
     if (a->ldx < a->D || a->lddt < a->D || a->ldb < (int64_t)a->G * a->N || a->ldc < (int64_t)a->G * a->N || (a->z && a->ldz < a->D)) return PSVAE_E_SHAPE;
     return 0;
 }
@@ -674,28 +786,38 @@ Scan scan_args(const psvae_scan* a, const Plan& p) {
     return q;
 }
 
-template <class T, int P, int K> int fwd_run(hipStream_t s, const Scan& q, const Plan& p) {
+template <class T, int P, int K, bool VEC> int fwd_run_as(hipStream_t s, const Scan& q, const Plan& p) {
     if (p.chunks > 1) {
-        hipLaunchKernelGGL((scan_fwd_kernel<T, P, K, true>), dim3(p.blocks, p.slots, p.chunks - 1), dim3(256), 0, s, q);
+        hipLaunchKernelGGL((scan_fwd_kernel<T, P, K, VEC, true>), dim3(p.blocks, p.slots, p.chunks - 1), dim3(256), 0, s, q);
         PSVAE_LAUNCH_CHECK();
     }
-    hipLaunchKernelGGL((scan_fwd_kernel<T, P, K, false>), dim3(p.blocks, p.slots, p.chunks + q.zero_outside), dim3(256), 0, s, q);
+    hipLaunchKernelGGL((scan_fwd_kernel<T, P, K, VEC, false>), dim3(p.blocks, p.slots, p.chunks + q.zero_outside), dim3(256), 0, s, q);
     PSVAE_LAUNCH_CHECK();
     return 0;
+}
+template <class T, int P, int K, bool VEC> int bwd_run_as(hipStream_t s, const Scan& q, const Plan& p) {
+    if (p.chunks > 1) {
+        hipLaunchKernelGGL((scan_bwd_kernel<T, P, K, VEC, true>), dim3(p.blocks, p.slots, p.chunks - 1), dim3(256), 0, s, q);
+        PSVAE_LAUNCH_CHECK();
+    }
+    hipLaunchKernelGGL((scan_bwd_kernel<T, P, K, VEC, false>), dim3(p.blocks, p.slots, p.chunks + q.zero_outside), dim3(256), 0, s, q);
+    PSVAE_LAUNCH_CHECK();
+    return 0;
+}
+template <class T, int P, int K> int fwd_run(hipStream_t s, const Scan& q, const Plan& p) {
+    return q.vec ? fwd_run_as<T, P, K, true>(s, q, p) : fwd_run_as<T, P, K, false>(s, q, p);
 }
 template <class T, int P, int K> int bwd_run(hipStream_t s, const Scan& q, const Plan& p) {
-    if (p.chunks > 1) {
-        hipLaunchKernelGGL((scan_bwd_kernel<T, P, K, true>), dim3(p.blocks, p.slots, p.chunks - 1), dim3(256), 0, s, q);
-        PSVAE_LAUNCH_CHECK();
-    }
-    hipLaunchKernelGGL((scan_bwd_kernel<T, P, K, false>), dim3(p.blocks, p.slots, p.chunks + q.zero_outside), dim3(256), 0, s, q);
-    PSVAE_LAUNCH_CHECK();
-    return 0;
+    return q.vec ? bwd_run_as<T, P, K, true>(s, q, p) : bwd_run_as<T, P, K, false>(s, q, p);
 }
 template <class T, int P, int K> int step_run(hipStream_t s, const Scan& q, const Plan&) {
-    const int64_t lanes = (int64_t)q.S * q.Dn * P;
     const int vec = q.N == P * K && rows_vec(q.A, 0, K, PSVAE_F32) && rows_vec(q.h0, 0, K, PSVAE_F32) && rows_vec(q.hT, 0, K, PSVAE_F32);
-    hipLaunchKernelGGL((scan_step_kernel<T, P, K>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, s, q, vec);
+    const int64_t wide = (q.Dn * P + 255) / 256;
+    // four sequences a lane where that leaves two workgroups for every CU
+    if (wide * ((q.S + 3) / 4) >= 512)
+        hipLaunchKernelGGL((scan_step_kernel<T, P, K, 4>), dim3((unsigned)(wide * ((q.S + 3) / 4))), dim3(256), 0, s, q, vec);
+    else
+        hipLaunchKernelGGL((scan_step_kernel<T, P, K, 1>), dim3((unsigned)(wide * q.S)), dim3(256), 0, s, q, vec);
     PSVAE_LAUNCH_CHECK();
     return 0;
 }
@@ -734,13 +856,13 @@ extern "C" size_t psvae_selective_scan_scratch_bytes(int64_t T, int S, int D, in
 
 extern "C" size_t psvae_selective_scan_saved_bytes(int64_t T, int S, int D, int G, int N) {
     if (!scan_sizes_ok(T, S, D, G, N, &T)) return 0;
-    return (size_t)(T / TILE + S) * D * scan_plan(T, S, D, G, N).NP * sizeof(float);
+    return (size_t)(T / HALF + S) * D * scan_plan(T, S, D, G, N).NP * sizeof(float);
 }
 
 extern "C" int psvae_selective_scan_forward(const psvae_scan* a, void* y, int64_t ldy, float* hT, void* saved, void* scratch,
                                             size_t scratch_bytes, void* stream) {
     PSVAE_TRY(scan_operands(a));
-    if (ldy < a->D) return PSVAE_E_SHAPE;
+    if (ldy < a->D || ldy >= 1 << 26) return PSVAE_E_SHAPE;
     if (a->T > 0 && !y) return PSVAE_E_NULL;
     if (a->S == 0) return 0;
     const Plan p = scan_plan(a->T, a->S, a->D, a->G, a->N);
@@ -765,7 +887,7 @@ extern "C" int psvae_selective_scan_backward(const psvae_scan* a, const void* sa
     if (!g) return PSVAE_E_NULL;
     if (a->T > 0 && (!saved || !dy || !g->dx || !g->ddt || !g->dB || !g->dC || (a->z && !g->dz))) return PSVAE_E_NULL;
     if (!g->dA || !scratch) return PSVAE_E_NULL;
-    if (lddy < a->D || g->lddx < a->D || g->ldddt < a->D || (a->z && g->lddz < a->D) || g->lddb < (int64_t)a->G * a->N || g->lddc < (int64_t)a->G * a->N) return PSVAE_E_SHAPE;
+    if (lddy < a->D || lddy >= 1 << 26) return PSVAE_E_SHAPE;
     const Plan p = scan_plan(a->T, a->S, a->D, a->G, a->N);
     Scan q = scan_args(a, p);
     const BwdScratch o = bwd_scratch(p, a->T, a->S, a->D, a->G);
@@ -773,25 +895,26 @@ extern "C" int psvae_selective_scan_backward(const psvae_scan* a, const void* sa
     if (scratch_bytes < o.total * sizeof(float)) return PSVAE_E_WORKSPACE;
     float* base = (float*)scratch;
     q.dy = dy; q.lddy = lddy; q.dhT = dhT; q.kept = (float*)saved;
-    q.dx = g->dx; q.lddx = g->lddx; q.ddt = g->ddt; q.ldddt = g->ldddt; q.dz = g->dz; q.lddz = g->lddz; q.dh0 = g->dh0;
+    q.dx = g->dx; q.ddt = g->ddt; q.dz = g->dz; q.dh0 = g->dh0;
     q.part_bc = base + o.bc; q.part_a = base + o.a; q.part_d = base + o.d;
     q.chunk_h = base + o.chunk;
     q.chunk_s = q.chunk_h + (size_t)(p.chunks - 1) * a->S * a->D * p.NP;
-    q.vec = q.vec && rows_vec(dy, lddy, p.VE, a->dtype) && rows_vec(g->dx, g->lddx, p.VE, a->dtype) &&
-            rows_vec(g->ddt, g->ldddt, p.VE, a->dtype) && (!a->z || rows_vec(g->dz, g->lddz, p.VE, a->dtype));
+    q.vec = q.vec && rows_vec(dy, lddy, p.VE, a->dtype) && rows_vec(g->dx, a->D, p.VE, a->dtype) &&
+            rows_vec(g->ddt, a->D, p.VE, a->dtype) && (!a->z || rows_vec(g->dz, a->D, p.VE, a->dtype));
     hipStream_t s = (hipStream_t)stream;
     ProfScope prof(s, KC_SCAN_BWD, (double)a->T * a->D * (a->z ? 7 : 5) * dtype_bytes(a->dtype));
     if (a->S > 0) {
         const int rc = PSVAE_SCAN_RUN(bwd_run, a->dtype, s, q, p);
         PSVAE_TRY(rc);
     }
-    ScanJoin j{q.part_bc, q.part_a, q.part_d, g->dB, g->dC, g->lddb, g->lddc, g->dA, g->d_skip, g->d_dt_bias, a->seq_off,
-               q.T, a->S, a->D, a->G, a->N, p.NP, p.tiles, a->S > 0 ? p.slots * p.chunks : 0, 0, 0, q.zero_outside};
+    ScanJoin j{q.part_bc, q.part_a, q.part_d, g->dB, g->dC, g->dA, g->d_skip, g->d_dt_bias, a->seq_off,
+               q.T, a->S, a->D, a->G, a->N, p.NP, p.tiles, a->S > 0 ? p.slots * p.chunks : 0, 0, 0, q.zero_outside, 0};
     const int64_t cols = (int64_t)a->T * a->G * 2 * p.NP;
-    j.blocks_bc = (int)((cols + 255) / 256 < 8192 ? (cols + 255) / 256 : 8192);
-    j.blocks_a = (int)(((int64_t)a->D * a->N + 255) / 256);
+    j.vec = a->N % 4 == 0 && rows_vec(g->dB, 0, 4, a->dtype) && rows_vec(g->dC, 0, 4, a->dtype);
+    j.blocks_bc = (int)((cols + 1023) / 1024 < 8192 ? (cols + 1023) / 1024 : 8192);
+    j.blocks_a = (int)(((int64_t)a->D * a->N + 63) / 64);
     PSVAE_BY_TYPE(a->dtype, T, {
-        hipLaunchKernelGGL((scan_join_kernel<T>), dim3(j.blocks_bc + j.blocks_a + (a->D + 255) / 256), dim3(256), 0, s, j);
+        hipLaunchKernelGGL((scan_join_kernel<T>), dim3(j.blocks_bc + j.blocks_a + (2 * a->D + 63) / 64), dim3(256), 0, s, j);
     });
     PSVAE_LAUNCH_CHECK();
     return 0;

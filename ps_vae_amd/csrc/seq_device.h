@@ -58,7 +58,8 @@ __device__ __forceinline__ float wave_add(float v) {
     return v;
 }
 
-__device__ __forceinline__ float sigmoidf(float v) { return __builtin_amdgcn_rcpf(1.f + expf(-v)); }
+// 1 / (1 + exp(-v)): off by |v| + 3 roundings, from the scaling of v
+__device__ __forceinline__ float sigmoidf(float v) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f)); }
 
 // Sequences of packed rows: offsets [S+1] in device memory, or (offsets null) S sequences of T / S rows.  Whatever the
 // offsets hold, the rows a sequence is given lie in [0, T).

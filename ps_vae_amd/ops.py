@@ -163,13 +163,24 @@ _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _l
 
 def _run(what, device, fn, *args):
     """The library call on the device's current stream, with that device current."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        # the handle alone: the Stream object of torch.cuda.current_stream() costs 2.7 us, as much as a launch
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, what)
+
+
+def _once(backward):
+    """A backward that cannot be differentiated again; the guard that says so is gone through only where somebody may."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 def _ptr(t):
@@ -258,7 +269,7 @@ class LayerNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         L = _lib.lib()
         x2, w, stats = ctx.saved_tensors
@@ -308,7 +319,7 @@ class CausalConvFn(torch.autograd.Function):
         return y, out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy, _):
         L = _lib.lib()
         x2, w, b, state, seq_off = ctx.saved_tensors
@@ -428,7 +439,7 @@ class SelectiveScanFn(torch.autograd.Function):
         return y, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy, dlast):
         L = _lib.lib()
         x, dt, A, B, C, D, z, bias, seq_off, kept = ctx.saved_tensors
@@ -447,8 +458,7 @@ class SelectiveScanFn(torch.autograd.Function):
         dx, ddt, dB, dC, dz = like(xs), like(xs), like(bs), like(cs), None if z is None else like(xs)
         dA, dD = like((width, N), f32), None if D is None else like(width, f32)
         dbias, dh0 = None if bias is None else like(width, f32), None if hs is None else like(hs, f32)
-        g = _lib.ScanGrads(_ptr(dx), _ptr(ddt), _ptr(dB), _ptr(dC), _ptr(dz), width, width, G * N, G * N, width, _ptr(dA), _ptr(dD), _ptr(dbias),
-                           _ptr(dh0))
+        g = _lib.ScanGrads(_ptr(dx), _ptr(ddt), _ptr(dB), _ptr(dC), _ptr(dz), _ptr(dA), _ptr(dD), _ptr(dbias), _ptr(dh0))
         nbytes = L.psvae_selective_scan_scratch_bytes(rows, S, width, G, N, 1)
         sc = _scratch(nbytes, dev)
         _run('psvae_selective_scan_backward', dev, L.psvae_selective_scan_backward, a, _ptr(kept), dy2.data_ptr(), lddy, _ptr(dlast), g, sc.data_ptr(),

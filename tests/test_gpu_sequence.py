@@ -319,7 +319,7 @@ def test_scan_and_conv_leave_or_zero_rows_outside_the_sequences():
         dA = torch.empty(D, N, device=DEV)
         a = _lib.Scan(x=x.data_ptr(), dt=x.data_ptr(), B=B.data_ptr(), C=B.data_ptr(), A=A.data_ptr(), ldx=D, lddt=D, ldb=N, ldc=N,
                       seq_off=off.data_ptr(), T=T, S=2, D=D, G=1, N=N, dtype=0, flags=_lib.SEQ_SOFTPLUS | flag)
-        g = _lib.ScanGrads(dx=dx.data_ptr(), ddt=ddt.data_ptr(), dB=dB.data_ptr(), dC=dC.data_ptr(), lddx=D, ldddt=D, lddb=N, lddc=N, dA=dA.data_ptr())
+        g = _lib.ScanGrads(dx=dx.data_ptr(), ddt=ddt.data_ptr(), dB=dB.data_ptr(), dC=dC.data_ptr(), dA=dA.data_ptr())
         _lib.check(L.psvae_selective_scan_forward(C.byref(a), y.data_ptr(), D, None, kept.data_ptr(), sc.data_ptr(), sc.numel(), st))
         _lib.check(L.psvae_selective_scan_backward(C.byref(a), kept.data_ptr(), x.data_ptr(), D, None, C.byref(g), sc.data_ptr(), sc.numel(), st))
         _lib.check(L.psvae_causal_conv_forward(x.data_ptr(), D, w.data_ptr(), None, yc.data_ptr(), D, off.data_ptr(), None, None, T, 2, D, 4, 0, flag, st))

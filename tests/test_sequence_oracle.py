@@ -103,7 +103,7 @@ def test_c_entry_points_refuse_bad_arguments():
         f = dict(x=p, dt=p, B=p, C=p, A=p, ldx=8, lddt=8, ldb=4, ldc=4, T=6, S=2, D=8, G=1, N=4, dtype=0, flags=2)
         return _lib.Scan(**{**f, **over})
     fwd = lambda **over: L.psvae_selective_scan_forward(scan(**over), p, 8, None, None, None, 0, None)  # noqa: E731
-    for bad in (dict(T=7), dict(N=0), dict(N=65, ldb=65, ldc=65), dict(G=3), dict(G=0), dict(D=0), dict(ldx=7), dict(ldb=3), dict(dtype=9), dict(flags=1),
+    for bad in (dict(T=7), dict(N=0), dict(N=65, ldb=65, ldc=65), dict(G=3), dict(G=0), dict(D=0), dict(ldx=7), dict(ldx=1 << 26), dict(ldb=3), dict(dtype=9), dict(flags=1),
                 dict(S=-1), dict(z=p, ldz=0)):
         assert fwd(**bad) == E_SHAPE, bad
     for bad in (dict(x=None), dict(A=None), dict(C=None)):
@@ -111,7 +111,7 @@ def test_c_entry_points_refuse_bad_arguments():
     assert L.psvae_selective_scan_forward(None, p, 8, None, None, None, 0, None) == E_NULL
     assert L.psvae_selective_scan_step(scan(T=6, S=2), p, 8, p, None) == E_SHAPE                               # T != S
     assert L.psvae_selective_scan_step(scan(T=2, S=2), p, 8, p, None) == E_NULL                                # no h0
-    g = _lib.ScanGrads(dx=p, ddt=p, dB=p, dC=p, dA=p, lddx=8, ldddt=8, lddb=4, lddc=4)
+    g = _lib.ScanGrads(dx=p, ddt=p, dB=p, dC=p, dA=p)
     n = L.psvae_selective_scan_scratch_bytes(6, 2, 8, 1, 4, 1)
     back = lambda scratch, nbytes, saved=p: L.psvae_selective_scan_backward(scan(), saved, p, 8, None, g, scratch, nbytes, None)  # noqa: E731
     assert back(p, n - 1) == E_WORKSPACE and back(p + 4, n) == E_ALIGN and back(p, n, None) == E_NULL and back(None, n) == E_NULL
@@ -122,7 +122,7 @@ def test_c_entry_points_refuse_bad_arguments():
         assert L.psvae_selective_scan_forward(scan(), p, 8, None, None, p, 16, None) == E_WORKSPACE
     finally:
         _lib.set_option('scan_chunks', old)
-    assert C.sizeof(_lib.Scan) == 8 * 15 + 8 + 24 and C.sizeof(_lib.ScanGrads) == 8 * 14
+    assert C.sizeof(_lib.Scan) == 8 * 15 + 8 + 24 and C.sizeof(_lib.ScanGrads) == 8 * 9
 
 
 def test_operators_refuse_cpu_tensors():
