@@ -42,6 +42,7 @@ __device__ __forceinline__ void input_row(const T* x, int64_t ldx, const T* stat
 }
 
 struct ConvShape { int T, D, S, R, lanes; int flags; };   // R rows a stretch, `lanes` lanes side by side in a row
+constexpr int GROUP = 4;   // rows loaded at a time, while the group before them is worked on
 
 template <class T, int V, int W>
 __global__ __launch_bounds__(256) void conv_fwd_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ w,
@@ -52,6 +53,15 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(const T* __restrict__ x, 
     if (c >= q.D || t0 >= q.T) return;
     const int t1 = min(t0 + q.R, q.T);
     float wv[W][V], bv[V], win[W][V];
+    Raw<T, V> now[GROUP], next[GROUP];
+    x += c;
+    y += c;
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int j = 0; j < GROUP; ++j)
+            if (t + j < t1) next[j].load(x + (int64_t)(t + j) * ldx);
+    };
+    fetch(t0);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         bv[i] = b ? b[c + i] : 0.f;
@@ -59,41 +69,48 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(const T* __restrict__ x, 
         for (int k = 0; k < W; ++k) wv[k][i] = w[(int64_t)(c + i) * W + k];
     }
     Walk at = walk_to(off, q.S, q.T, t0);
+    auto run_up = [&](int t) {
 #pragma unroll
-    for (int k = 0; k + 1 < W; ++k) input_row<T, V>(x, ldx, state, at, t0 - W + 1 + k, W - 1, q.D, c, win[k + 1]);
-    for (int tb = t0; tb < t1; tb += 4) {
-        float next[4][V];                               // four rows in flight before the first is used
+        for (int k = 0; k + 1 < W; ++k) input_row<T, V>(x - c, ldx, state, at, t - W + 1 + k, W - 1, q.D, c, win[k + 1]);
+    };
+    auto row = [&](int t, const Raw<T, V>& in) {
+        float o[V];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (tb + j < t1) load_vec<V>(x + (int64_t)(tb + j) * ldx + c, next[j]);
+        for (int i = 0; i < V; ++i) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+            for (int k = 0; k + 1 < W; ++k) win[k][i] = win[k + 1][i];
+            win[W - 1][i] = in[i];
+            float pre = bv[i];
+#pragma unroll
+            for (int k = 0; k < W; ++k) pre = fmaf(wv[k][i], win[k][i], pre);
+            o[i] = q.flags & PSVAE_SEQ_SILU ? pre * sigmoidf(pre) : pre;
+        }
+        store_vec<V>(y + (int64_t)t * ldy, o);
+    };
+    run_up(t0);
+    for (int tb = t0; tb < t1; tb += GROUP) {
+#pragma unroll
+        for (int j = 0; j < GROUP; ++j) now[j] = next[j];
+        fetch(tb + GROUP);
+        if (tb > at.begin && tb + GROUP <= min(at.end, t1)) {
+#pragma unroll
+            for (int j = 0; j < GROUP; ++j) row(tb + j, now[j]);
+            continue;
+        }
+#pragma unroll
+        for (int j = 0; j < GROUP; ++j) {               // a border of a sequence or of the stretch lies in this group
             const int t = tb + j;
             if (t >= t1) break;
             if (t >= at.end && at.s < q.S) at = walk_to(off, q.S, q.T, t);   // the next sequence that has rows, or none
-            if (t == at.begin) {
+            if (t == at.begin) run_up(t);
+            if (at.s < q.S && t >= at.begin) {
+                row(t, now[j]);
+            } else if (q.flags & PSVAE_SEQ_ZERO_OUTSIDE) {
+                float zero[V];
 #pragma unroll
-                for (int k = 0; k + 1 < W; ++k) input_row<T, V>(x, ldx, state, at, t - W + 1 + k, W - 1, q.D, c, win[k + 1]);
+                for (int i = 0; i < V; ++i) zero[i] = 0.f;
+                store_vec<V>(y + (int64_t)t * ldy, zero);
             }
-            float o[V];
-            if (at.s >= q.S || t < at.begin) {
-                if (!(q.flags & PSVAE_SEQ_ZERO_OUTSIDE)) continue;
-#pragma unroll
-                for (int i = 0; i < V; ++i) o[i] = 0.f;
-                store_vec<V>(y + (int64_t)t * ldy + c, o);
-                continue;
-            }
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-#pragma unroll
-                for (int k = 0; k + 1 < W; ++k) win[k][i] = win[k + 1][i];
-                win[W - 1][i] = next[j][i];
-                float pre = bv[i];
-#pragma unroll
-                for (int k = 0; k < W; ++k) pre = fmaf(wv[k][i], win[k][i], pre);
-                o[i] = q.flags & PSVAE_SEQ_SILU ? pre * sigmoidf(pre) : pre;
-            }
-            store_vec<V>(y + (int64_t)t * ldy + c, o);
         }
     }
 }
@@ -142,21 +159,63 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(const T* __restrict__ dy,
             if (dx && row >= t0 && row < t1) store_vec<V>(dx + (int64_t)row * lddx + c, g);
         };
         Walk at = walk_to(off, q.S, q.T, t0);
+        const int last = min(t1 + W - 1, q.T);          // rows behind the stretch that its own rows' gradients come from, too
+        Raw<T, V> xr[GROUP], gr[GROUP], xn[GROUP], gn[GROUP];
+        auto fetch = [&](int t) {
 #pragma unroll
-        for (int k = 0; k + 1 < W; ++k) input_row<T, V>(x, ldx, state, at, t0 - W + 1 + k, W - 1, q.D, c, win[k + 1]);
-        const int last = min(t1 + W - 1, q.T);
-        bool done = false;
-        int t = t0;
-        for (; t < last && !done;) {
-            float nx[2][V], ng[2][V];
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < GROUP; ++j)
                 if (t + j < last) {
-                    load_vec<V>(x + (int64_t)(t + j) * ldx + c, nx[j]);
-                    load_vec<V>(dy + (int64_t)(t + j) * lddy + c, ng[j]);
+                    xn[j].load(x + (int64_t)(t + j) * ldx + c);
+                    gn[j].load(dy + (int64_t)(t + j) * lddy + c);
                 }
+        };
+        auto run_up = [&](int t) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int k = 0; k + 1 < W; ++k) input_row<T, V>(x, ldx, state, at, t - W + 1 + k, W - 1, q.D, c, win[k + 1]);
+        };
+        auto row = [&](const Raw<T, V>& xin, const Raw<T, V>& gin, bool own) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+#pragma unroll
+                for (int k = 0; k + 1 < W; ++k) win[k][i] = win[k + 1][i];
+                win[W - 1][i] = xin[i];
+                float g = gin[i];
+                if (q.flags & PSVAE_SEQ_SILU) {
+                    float pre = bv[i];
+#pragma unroll
+                    for (int k = 0; k < W; ++k) pre = fmaf(wv[k][i], win[k][i], pre);
+                    const float sg = sigmoidf(pre);
+                    g *= sg * (1.f + pre * (1.f - sg));
+                }
+                // shift the ring down by one row, then give every row of the window its product
+#pragma unroll
+                for (int k = 0; k + 1 < W; ++k) ring[k][i] = fmaf(wv[k][i], g, ring[k + 1][i]);
+                ring[W - 1][i] = wv[W - 1][i] * g;
+                if (own) {
+                    db[i] += g;
+#pragma unroll
+                    for (int k = 0; k < W; ++k) dw[k][i] = fmaf(g, win[k][i], dw[k][i]);
+                }
+            }
+        };
+        fetch(t0);
+        run_up(t0);
+        bool done = false;
+        for (int tb = t0; tb < last && !done; tb += GROUP) {
+#pragma unroll
+            for (int j = 0; j < GROUP; ++j) { xr[j] = xn[j]; gr[j] = gn[j]; }
+            fetch(tb + GROUP);
+            if (tb - W + 1 >= max(t0, at.begin) && tb > at.begin && tb + GROUP <= min(at.end, t1)) {
+#pragma unroll
+                for (int j = 0; j < GROUP; ++j) {
+                    row(xr[j], gr[j], true);
+                    if (dx) store_vec<V>(dx + (int64_t)(tb + j - W + 1) * lddx + c, ring[0]);
+                }
+                continue;
+            }
+#pragma unroll
+            for (int j = 0; j < GROUP; ++j) {
+                const int t = tb + j;
                 if (t >= last || done) break;
                 if (t >= at.end && at.s < q.S) {
                     // the sequence is over: its last W - 1 rows have all that they get
@@ -170,10 +229,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(const T* __restrict__ dy,
                     if (t >= t1) { done = true; break; }
                     at = walk_to(off, q.S, q.T, t);
                 }
-                if (t == at.begin) {
-#pragma unroll
-                    for (int k = 0; k + 1 < W; ++k) input_row<T, V>(x, ldx, state, at, t - W + 1 + k, W - 1, q.D, c, win[k + 1]);
-                }
+                if (t == at.begin) run_up(t);
                 if (at.s >= q.S || t < at.begin) {
                     if (q.flags & PSVAE_SEQ_ZERO_OUTSIDE) {
                         float zero[V];
@@ -181,42 +237,17 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(const T* __restrict__ dy,
                         for (int i = 0; i < V; ++i) zero[i] = 0.f;
                         emit(t, zero);
                     }
-                    ++t;
                     continue;
                 }
-                float g[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-#pragma unroll
-                    for (int k = 0; k + 1 < W; ++k) win[k][i] = win[k + 1][i];
-                    win[W - 1][i] = nx[j][i];
-                    g[i] = ng[j][i];
-                    if (q.flags & PSVAE_SEQ_SILU) {
-                        float pre = bv[i];
-#pragma unroll
-                        for (int k = 0; k < W; ++k) pre = fmaf(wv[k][i], win[k][i], pre);
-                        const float sg = sigmoidf(pre);
-                        g[i] *= sg * (1.f + pre * (1.f - sg));
-                    }
-                    // shift the ring down by one row, then give every row of the window its product
-#pragma unroll
-                    for (int k = 0; k + 1 < W; ++k) ring[k][i] = fmaf(wv[k][i], g[i], ring[k + 1][i]);
-                    ring[W - 1][i] = wv[W - 1][i] * g[i];
-                    if (t < t1) {
-                        db[i] += g[i];
-#pragma unroll
-                        for (int k = 0; k < W; ++k) dw[k][i] = fmaf(g[i], win[k][i], dw[k][i]);
-                    }
-                }
+                row(xr[j], gr[j], t < t1);
                 if (t - W + 1 >= at.begin) emit(t - W + 1, ring[0]);
-                ++t;
             }
         }
-        // the walk ended inside a sequence or at its end: what is still in the ring is complete only if no row follows
-        if (!done && t >= q.T && at.s < q.S)
+        // the walk ended behind the last row: what is still in the ring is complete
+        if (!done && last == q.T && at.s < q.S)
 #pragma unroll
             for (int k = 1; k < W; ++k)
-                if (t - W + k >= at.begin && t - W + k < at.end) emit(t - W + k, ring[k]);
+                if (q.T - W + k >= at.begin && q.T - W + k < at.end) emit(q.T - W + k, ring[k]);
     }
     if (!partial) return;
     // join the stretches of this workgroup, one quantity after the other, in the stretches' order
@@ -276,9 +307,9 @@ int conv_rows(int64_t T, int nvec, int lanes) {
     while (R > 8 && (T + R * (256 / lanes) - 1) / (R * (256 / lanes)) * ((nvec + lanes - 1) / lanes) < 1024) R /= 2;
     return R;
 }
-// Channels of a lane: 16 bytes where rows allow vectors; half of it for more than four taps of a 16-bit type, whose
-// windows would not fit the registers.
-int conv_vec(int dtype, int W) { return dtype == PSVAE_F32 ? 4 : (W <= 4 ? 8 : 4); }
+// Channels of a lane where rows allow vectors: 16 bytes forward; four backward and for more than four taps, whose windows,
+// filters and sums would otherwise leave registers for a single wave of a SIMD.
+int conv_vec(int dtype, int W, bool backward) { return dtype == PSVAE_F32 || backward || W > 4 ? 4 : 8; }
 
 struct ConvPlan { ConvShape q; int V, gx, gy; };
 ConvPlan conv_plan(int64_t T, int D, int S, int V, int flags) {
@@ -295,13 +326,6 @@ template <class T, int V, int W> struct ConvRun {
         PSVAE_LAUNCH_CHECK();
         return 0;
     }
-    static int bwd(hipStream_t s, const ConvPlan& p, const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* w,
-                   const float* b, void* dx, int64_t lddx, float* partial, const int32_t* off, const void* state) {
-        hipLaunchKernelGGL((conv_bwd_kernel<T, V, W>), dim3(p.gx, p.gy), dim3(256), partial ? 256 * V * sizeof(float) : 0, s, (const T*)dy,
-                           lddy, (const T*)x, ldx, w, b, (T*)dx, lddx, partial, off, (const T*)state, p.q);
-        PSVAE_LAUNCH_CHECK();
-        return 0;
-    }
     static int step(hipStream_t s, const void* x, int64_t ldx, const void* state, void* state_out, const float* w, const float* b, void* y,
                     int64_t ldy, int S, int D, int flags) {
         const int64_t n = (int64_t)S * (D / V);
@@ -310,25 +334,38 @@ template <class T, int V, int W> struct ConvRun {
         PSVAE_LAUNCH_CHECK();
         return 0;
     }
+    static int bwd(hipStream_t s, const ConvPlan& p, const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* w,
+                   const float* b, void* dx, int64_t lddx, float* partial, const int32_t* off, const void* state) {
+        hipLaunchKernelGGL((conv_bwd_kernel<T, V, W>), dim3(p.gx, p.gy), dim3(256), partial ? 256 * V * sizeof(float) : 0, s, (const T*)dy,
+                           lddy, (const T*)x, ldx, w, b, (T*)dx, lddx, partial, off, (const T*)state, p.q);
+        PSVAE_LAUNCH_CHECK();
+        return 0;
+    }
 };
 
-// Calls `call` of the ConvRun for (type, vector width, taps).
-#define PSVAE_CONV_TAPS(T, V, W, call)                         \
-    switch (W) {                                               \
-        case 1: return ConvRun<T, V, 1>::call;                 \
-        case 2: return ConvRun<T, V, 2>::call;                 \
-        case 3: return ConvRun<T, V, 3>::call;                 \
-        case 4: return ConvRun<T, V, 4>::call;                 \
-        case 5: return ConvRun<T, (V > 4 ? 4 : V), 5>::call;   \
-        case 6: return ConvRun<T, (V > 4 ? 4 : V), 6>::call;   \
-        case 7: return ConvRun<T, (V > 4 ? 4 : V), 7>::call;   \
-        default: return ConvRun<T, (V > 4 ? 4 : V), 8>::call;  \
+// Calls `call` of the ConvRun for (type, vector width V, taps).
+#define PSVAE_CONV_TAPS(T, V, W, call)                 \
+    switch (W) {                                       \
+        case 1: return ConvRun<T, V, 1>::call;         \
+        case 2: return ConvRun<T, V, 2>::call;         \
+        case 3: return ConvRun<T, V, 3>::call;         \
+        case 4: return ConvRun<T, V, 4>::call;         \
+        case 5: return ConvRun<T, min4(V), 5>::call;   \
+        case 6: return ConvRun<T, min4(V), 6>::call;   \
+        case 7: return ConvRun<T, min4(V), 7>::call;   \
+        default: return ConvRun<T, min4(V), 8>::call;  \
     }
-#define PSVAE_CONV_RUN(dtype, vec, W, call)                    \
-    PSVAE_BY_TYPE(dtype, T, {                                  \
-        if (vec) { PSVAE_CONV_TAPS(T, (int)(16 / sizeof(T)), W, call) } \
-        else { PSVAE_CONV_TAPS(T, 1, W, call) }                \
+#define PSVAE_CONV_RUN(dtype, V, W, call)                                    \
+    PSVAE_BY_TYPE(dtype, T, {                                                \
+        if ((V) == 1) { PSVAE_CONV_TAPS(T, 1, W, call) }                     \
+        else { PSVAE_CONV_TAPS(T, (int)(16 / sizeof(T)), W, call) }          \
     })
+#define PSVAE_CONV_RUN4(dtype, V, W, call)                                   \
+    PSVAE_BY_TYPE(dtype, T, {                                                \
+        if ((V) == 1) { PSVAE_CONV_TAPS(T, 1, W, call) }                     \
+        else { PSVAE_CONV_TAPS(T, 4, W, call) }                              \
+    })
+constexpr int min4(int v) { return v < 4 ? v : 4; }
 
 bool conv_sizes_ok(int64_t T, int S, int D, int W, int dtype, const void* off) {
     if (T < 0 || T > INT32_MAX - 64 * 64 || S < 0 || D < 1 || D > (1 << 21) || W < 1 || W > 8 || !dtype_known(dtype)) return false;
@@ -354,15 +391,15 @@ extern "C" int psvae_causal_conv_forward(const void* x, int64_t ldx, const float
         PSVAE_LAUNCH_CHECK();
     }
     if (T == 0) return 0;
-    const int V = conv_vec(dtype, W);
+    const int V = conv_vec(dtype, W, false);
     const bool vec = D % V == 0 && rows_vec(x, ldx, V, dtype) && rows_vec(y, ldy, V, dtype) && rows_vec(state, D, V, dtype);
     const ConvPlan p = conv_plan(T, D, S, vec ? V : 1, flags);
-    PSVAE_CONV_RUN(dtype, vec, W, fwd(s, p, x, ldx, weight, bias, y, ldy, seq_off, state));
+    PSVAE_CONV_RUN(dtype, p.V, W, fwd(s, p, x, ldx, weight, bias, y, ldy, seq_off, state));
 }
 
 extern "C" size_t psvae_causal_conv_scratch_bytes(int64_t T, int D, int W, int dtype) {
     if (!conv_sizes_ok(T, 1, D, W, dtype, nullptr)) return 0;
-    const ConvPlan a = conv_plan(T, D, 1, conv_vec(dtype, W), 0), b = conv_plan(T, D, 1, 1, 0);   // either may be taken
+    const ConvPlan a = conv_plan(T, D, 1, 4, 0), b = conv_plan(T, D, 1, 1, 0);   // either may be taken
     return (size_t)((a.gx > b.gx ? a.gx : b.gx) + 1) * (W + 1) * D * sizeof(float);
 }
 
@@ -384,13 +421,13 @@ extern "C" int psvae_causal_conv_backward(const void* dy, int64_t lddy, const vo
     float* partial = params ? (float*)scratch : nullptr;
     int parts = 0;
     if (T > 0) {
-        const int V = conv_vec(dtype, W);
+        const int V = conv_vec(dtype, W, true);
         const bool vec = D % V == 0 && rows_vec(x, ldx, V, dtype) && rows_vec(dy, lddy, V, dtype) && rows_vec(dx, lddx, V, dtype) &&
                          rows_vec(state, D, V, dtype);
         const ConvPlan p = conv_plan(T, D, S, vec ? V : 1, flags);
         parts = p.gx;
         const int rc = [&]() -> int {
-            PSVAE_CONV_RUN(dtype, vec, W, bwd(s, p, dy, lddy, x, ldx, weight, bias, dx, lddx, partial, seq_off, state));
+            PSVAE_CONV_RUN4(dtype, p.V, W, bwd(s, p, dy, lddy, x, ldx, weight, bias, dx, lddx, partial, seq_off, state));
         }();
         PSVAE_TRY(rc);
     }
@@ -402,9 +439,9 @@ extern "C" int psvae_causal_conv_step(const void* x, int64_t ldx, const void* st
     if (S < 0 || D < 1 || D > (1 << 21) || W < 1 || W > 8 || !dtype_known(dtype) || ldx < D || ldy < D || (flags & ~PSVAE_SEQ_SILU)) return PSVAE_E_SHAPE;
     if (S == 0) return 0;
     if (!x || !weight || !y || (W > 1 && (!state || !state_out))) return PSVAE_E_NULL;
-    const int V = conv_vec(dtype, W);
+    const int V = conv_vec(dtype, W, false);
     const bool vec = D % V == 0 && rows_vec(x, ldx, V, dtype) && rows_vec(y, ldy, V, dtype) && rows_vec(state, D, V, dtype) && rows_vec(state_out, D, V, dtype);
     hipStream_t s = (hipStream_t)stream;
     ProfScope prof(s, KC_SEQ_CONV, 2.0 * S * D * W * dtype_bytes(dtype));
-    PSVAE_CONV_RUN(dtype, vec, W, step(s, x, ldx, state, state_out, weight, bias, y, ldy, S, D, flags));
+    PSVAE_CONV_RUN(dtype, vec ? V : 1, W, step(s, x, ldx, state, state_out, weight, bias, y, ldy, S, D, flags));
 }

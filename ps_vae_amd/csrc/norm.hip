@@ -135,17 +135,31 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(const T* __restrict__ dy,
         if (w && c < H) load_vec<V>(w + c, wv[i]);
     }
     const float inv = 1.f / (float)H;
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + (WPR == 1 ? wave : 0); row < rows; row += (int64_t)gridDim.x * ROWS) {
-        const float mu = mean[row], rs = rstd[row];
-        float g[IT][V], xh[IT][V], s0 = 0.f, s1 = 0.f;
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    Raw<T, V> gn[IT], xn[IT];                          // the next row, on its way while this one is worked on
+    float mun = 0.f, rsn = 0.f;
+    auto fetch = [&](int64_t row) {
+        mun = mean[row];
+        rsn = rstd[row];
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int c = (i * 64 * WPR + lane) * V;
             if (c < H) {
-                load_vec<V>(dy + row * lddy + c, g[i]);
-                load_vec<V>(x + row * ldx + c, xh[i]);
+                gn[i].load(dy + row * lddy + c);
+                xn[i].load(x + row * ldx + c);
             }
         }
+    };
+    int64_t row = (int64_t)blockIdx.x * ROWS + (WPR == 1 ? wave : 0);
+    if (row < rows) fetch(row);
+    for (; row < rows; row += step) {
+        const float mu = mun, rs = rsn;
+        float g[IT][V], xh[IT][V], s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
+#pragma unroll
+            for (int k = 0; k < V; ++k) { g[i][k] = gn[i][k]; xh[i][k] = xn[i][k]; }
+        if (row + step < rows) fetch(row + step);
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int c = (i * 64 * WPR + lane) * V;
@@ -280,6 +294,7 @@ __global__ __launch_bounds__(256) void column_sums_kernel(const float* __restric
     const int c = blockIdx.x * 16 + cx;
     float s = 0.f;
     if (c < columns)
+#pragma unroll 8
         for (int p = px; p < parts; p += 16) s += partial[(int64_t)p * columns + c];
     red[px][cx] = s;
     __syncthreads();

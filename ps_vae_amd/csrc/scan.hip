@@ -125,9 +125,8 @@ __device__ __forceinline__ int64_t kept_row(int begin, int s, int tile) { return
 // that the 16 lanes that write one row of 64 (or 32) channels reach as many bank groups.
 __device__ __forceinline__ int quarter(int q, int ch) { return 4 * (q ^ (ch >> 4 & 3)); }
 
-// V elements in the type they are stored in, so that a prefetch waits for nothing.  `base` is the same for the workgroup,
-// the lane's distance from it fits 32 bits (rows lie less than 2^26 elements apart).
-template <class T, int V> struct Raw { T v[V]; };
+// V elements of a row, zeros from the n-th on.  `base` is the same for the workgroup, the lane's distance from it fits 32
+// bits (rows lie less than 2^26 elements apart).
 template <bool VEC, class T, int V>
 __device__ __forceinline__ void fetch_row(const void* base, unsigned offset, int n, Raw<T, V>& out) {
     asm volatile("" : "+v"(offset));       // keeps base + offset in the instruction: hoisted sums would fill the registers
@@ -693,12 +692,8 @@ template <class T, int P, int K, int R> __global__ __launch_bounds__(256) void s
         x[i] = (float)((const T*)q.x)[s * q.ldx + d];
         v[i] = (float)((const T*)q.dt)[s * q.lddt + d] + bias;
         z[i] = q.z ? (float)((const T*)q.z)[s * q.ldz + d] : 0.f;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int n = n0 + k < q.N ? n0 + k : 0;
-            b[i][k] = (float)((const T*)q.B)[s * q.ldb + g * q.N + n];
-            c[i][k] = n0 + k < q.N ? (float)((const T*)q.C)[s * q.ldc + g * q.N + n] : 0.f;
-        }
+        load_some<K>((const T*)q.B + s * q.ldb + g * q.N + n0, q.N - n0, q.vec, b[i]);
+        load_some<K>((const T*)q.C + s * q.ldc + g * q.N + n0, q.N - n0, q.vec, c[i]);
     }
     if (vec_state) load_vec<K>(q.A + (int64_t)d * q.N + n0, A);
     else load_state<K>(q.A, 0, q, d, n0, A);
@@ -928,6 +923,7 @@ extern "C" int psvae_selective_scan_step(const psvae_scan* a, void* y, int64_t l
     const Plan p = scan_plan(a->T, a->S, a->D, a->G, a->N);
     Scan q = scan_args(a, p);
     q.y = y; q.ldy = ldy; q.hT = hT;
+    q.vec = a->N % p.K == 0 && rows_vec(a->B, a->ldb, p.K, a->dtype) && rows_vec(a->C, a->ldc, p.K, a->dtype);   // of B and C
     hipStream_t s = (hipStream_t)stream;
     ProfScope prof(s, KC_SCAN_FWD, (double)a->S * a->D * a->N * 8);
     return PSVAE_SCAN_RUN(step_run, a->dtype, s, q, p);

@@ -52,6 +52,16 @@ template <int V, class T> __device__ __forceinline__ void store_some(T* p, int n
     }
 }
 
+// V elements in the type they are stored in: what a prefetch loads, so that nothing waits for it before it is used.
+template <class T, int V> struct Raw {
+    typename VecOf<T, V>::type v;
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (V == 1) v[0] = p[0];
+        else v = *(const typename VecOf<T, V>::type*)p;
+    }
+    __device__ __forceinline__ float operator[](int i) const { return (float)v[i]; }
+};
+
 __device__ __forceinline__ float wave_add(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);

@@ -201,7 +201,7 @@ def _act(what, name, t, like, shape):
     """Checks an activation operand against the call's first one."""
     if t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f'{what}: {name} is {t.dtype} on {t.device}, x is {like.dtype} on {like.device}')
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f'{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}')
 
 
@@ -209,20 +209,22 @@ def _par(what, name, t, like, shape):
     """A parameter or state: checked, fp32, contiguous."""
     if t is None:
         return None
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f'{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}')
     if t.device != like.device:
         raise ValueError(f'{what}: {name} is on {t.device}, x is on {like.device}')
+    if t.dtype is torch.float32:
+        return t if t.is_contiguous() else t.contiguous()
     if not t.is_floating_point():
         raise ValueError(f'{what}: {name} is {t.dtype}, expected a floating type')
-    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
+    return t.float().contiguous()
 
 
-def _first(what, x, dims):
+def _first(what, x, low, high):
     _need_gpu(x, what)
     if x.dtype not in _DTYPES:
         raise ValueError(f'{what}: x is {x.dtype}; float32, bfloat16 and float16 are supported')
-    if x.dim() not in dims:
+    if not low <= x.dim() <= high:
         raise ValueError(f'{what}: x has {x.dim()} dimensions')
     if x.shape[-1] < 1:
         raise ValueError(f'{what}: x has no channels')
@@ -235,7 +237,7 @@ def _sequences(what, x, seq_off):
         return rows, (1 if x.dim() == 2 else x.shape[0])
     if x.dim() != 2:
         raise ValueError(f'{what}: seq_off goes with packed rows [T, width], x has {x.dim()} dimensions')
-    if seq_off.dtype != torch.int32 or seq_off.dim() != 1 or seq_off.numel() < 1 or not seq_off.is_contiguous() or seq_off.device != x.device:
+    if seq_off.dtype is not torch.int32 or seq_off.dim() != 1 or not seq_off.is_contiguous() or seq_off.device != x.device or not len(seq_off):
         raise ValueError(f'{what}: seq_off must be a contiguous int32 vector of sequences + 1 offsets on {x.device}')
     if seq_off.numel() == 1 and rows:
         raise ValueError(f'{what}: seq_off names no sequence for {rows} rows')
@@ -243,18 +245,25 @@ def _sequences(what, x, seq_off):
 
 
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _norm_forward(x, w, b, eps, keep):
-    H = x.shape[-1]
+    H, dev = x.shape[-1], x.device
     rows = x.numel() // H
     x2, ldx = _rows(x, H)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if keep else None
-    at = stats.data_ptr() if keep else None
-    _run('psvae_layer_norm_forward', x.device, _lib.lib().psvae_layer_norm_forward, x2.data_ptr(), ldx, _ptr(w), _ptr(b), y.data_ptr(), H,
-         at, at + 4 * rows if keep else None, rows, H, eps, _DTYPES[x.dtype])
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    stats, mean, rstd = None, None, None
+    if keep:
+        stats = torch.empty(2, rows, dtype=torch.float32, device=dev)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * rows
+    _run('psvae_layer_norm_forward', dev, _lib.lib().psvae_layer_norm_forward, x2.data_ptr(), ldx, _ptr(w), _ptr(b), y.data_ptr(), H, mean, rstd,
+         rows, H, eps, _DTYPES[x.dtype])
     return y, x2, ldx, stats
 
 
@@ -265,7 +274,7 @@ class LayerNormFn(torch.autograd.Function):
     def forward(ctx, x, w, b, eps):
         y, x2, ctx.ldx, stats = _norm_forward(x, w, b, eps, True)
         ctx.save_for_backward(x2, w, stats)
-        ctx.has_bias, ctx.shape = b is not None, x.shape
+        ctx.shape = x.shape
         return y
 
     @staticmethod
@@ -273,35 +282,37 @@ class LayerNormFn(torch.autograd.Function):
     def backward(ctx, dy):
         L = _lib.lib()
         x2, w, stats = ctx.saved_tensors
-        H, rows = ctx.shape[-1], stats.shape[1]
-        need_x, need_w, need_b = ctx.needs_input_grad[0], w is not None and ctx.needs_input_grad[1], ctx.has_bias and ctx.needs_input_grad[2]
+        need_x, need_w, need_b, _ = ctx.needs_input_grad      # False where the operand was None
+        shape, rows, dev, dtype = ctx.shape, stats.shape[1], stats.device, x2.dtype
+        H = shape[-1]
         dy2, lddy = _rows(dy, H)
-        dev = dy.device
-        dx = torch.empty(ctx.shape, dtype=x2.dtype, device=dev) if need_x else None
+        dx = torch.empty(shape, dtype=dtype, device=dev) if need_x else None
         dw = torch.empty(H, dtype=torch.float32, device=dev) if need_w else None
         db = torch.empty(H, dtype=torch.float32, device=dev) if need_b else None
-        sc = _scratch(L.psvae_layer_norm_scratch_bytes(rows, H), dev) if need_w or need_b else None
-        _run('psvae_layer_norm_backward', dev, L.psvae_layer_norm_backward, dy2.data_ptr(), lddy, x2.data_ptr(), ctx.ldx, _ptr(w), stats.data_ptr(),
-             stats.data_ptr() + 4 * rows, _ptr(dx), H, _ptr(dw), _ptr(db), rows, H, _DTYPES[x2.dtype], _ptr(sc), sc.numel() if sc is not None else 0)
+        nbytes = L.psvae_layer_norm_scratch_bytes(rows, H) if need_w or need_b else 0
+        sc = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        mean = stats.data_ptr()
+        _run('psvae_layer_norm_backward', dev, L.psvae_layer_norm_backward, dy2.data_ptr(), lddy, x2.data_ptr(), ctx.ldx, _ptr(w), mean,
+             mean + 4 * rows, _ptr(dx), H, _ptr(dw), _ptr(db), rows, H, _DTYPES[dtype], _ptr(sc), nbytes)
         return dx, dw, db, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer norm over the last dimension of x [.., H]; weight and bias [H], each optional."""
-    _first('layer_norm', x, range(1, 65))
-    H = x.shape[-1]
-    weight, bias = _par('layer_norm', 'weight', weight, x, (H,)), _par('layer_norm', 'bias', bias, x, (H,))
+    _first('layer_norm', x, 1, 64)
+    shape = x.shape[-1:]
+    weight, bias = _par('layer_norm', 'weight', weight, x, shape), _par('layer_norm', 'bias', bias, x, shape)
     if _wants_grad(x, weight, bias):
         return LayerNormFn.apply(x, weight, bias, float(eps))
     return _norm_forward(x, weight, bias, float(eps), False)[0]
 
 
 def _conv_forward(x, w, b, state, seq_off, flags, rows, S, want_state):
-    D, W = w.shape
+    (D, W), dev = w.shape, x.device
     x2, ldx = _rows(x, D)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    out = torch.empty(S, W - 1, D, dtype=x.dtype, device=x.device) if want_state else None
-    _run('psvae_causal_conv_forward', x.device, _lib.lib().psvae_causal_conv_forward, x2.data_ptr(), ldx, w.data_ptr(), _ptr(b), y.data_ptr(), D,
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    out = torch.empty(S, W - 1, D, dtype=x.dtype, device=dev) if want_state else None
+    _run('psvae_causal_conv_forward', dev, _lib.lib().psvae_causal_conv_forward, x2.data_ptr(), ldx, w.data_ptr(), _ptr(b), y.data_ptr(), D,
          _ptr(seq_off), _ptr(state), _ptr(out), rows, S, D, W, _DTYPES[x.dtype], flags)
     return y, out, x2, ldx
 
@@ -311,9 +322,9 @@ class CausalConvFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, b, state, seq_off, flags, rows, S, want_state):
-        y, out, x2, ctx.ldx = _conv_forward(x, w, b, state, seq_off, flags, rows, S, want_state)
+        y, out, x2, ldx = _conv_forward(x, w, b, state, seq_off, flags, rows, S, want_state)
         ctx.save_for_backward(x2, w, b, state, seq_off)
-        ctx.flags, ctx.rows, ctx.S, ctx.shape = flags, rows, S, x.shape
+        ctx.call = ldx, flags, rows, S, x.shape
         if out is not None:
             ctx.mark_non_differentiable(out)
         return y, out
@@ -323,18 +334,18 @@ class CausalConvFn(torch.autograd.Function):
     def backward(ctx, dy, _):
         L = _lib.lib()
         x2, w, b, state, seq_off = ctx.saved_tensors
-        D, W = w.shape
-        dev = dy.device
-        need_x, need_w, need_b = ctx.needs_input_grad[0], ctx.needs_input_grad[1], b is not None and ctx.needs_input_grad[2]
+        ldx, flags, rows, S, shape = ctx.call
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]     # False where the operand was None
+        (D, W), dev, dtype = w.shape, w.device, x2.dtype
         dy2, lddy = _rows(dy, D)
-        dx = torch.empty(ctx.shape, dtype=x2.dtype, device=dev) if need_x else None
+        dx = torch.empty(shape, dtype=dtype, device=dev) if need_x else None
         dw = torch.empty(D, W, dtype=torch.float32, device=dev) if need_w else None
         db = torch.empty(D, dtype=torch.float32, device=dev) if need_b else None
-        dtype = _DTYPES[x2.dtype]
-        sc = _scratch(L.psvae_causal_conv_scratch_bytes(ctx.rows, D, W, dtype), dev) if need_w or need_b else None
-        _run('psvae_causal_conv_backward', dev, L.psvae_causal_conv_backward, dy2.data_ptr(), lddy, x2.data_ptr(), ctx.ldx, w.data_ptr(), _ptr(b),
-             _ptr(dx), D, _ptr(dw), _ptr(db), _ptr(seq_off), _ptr(state), ctx.rows, ctx.S, D, W, dtype, ctx.flags, _ptr(sc),
-             sc.numel() if sc is not None else 0)
+        code = _DTYPES[dtype]
+        nbytes = L.psvae_causal_conv_scratch_bytes(rows, D, W, code) if need_w or need_b else 0
+        sc = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _run('psvae_causal_conv_backward', dev, L.psvae_causal_conv_backward, dy2.data_ptr(), lddy, x2.data_ptr(), ldx, w.data_ptr(), _ptr(b),
+             _ptr(dx), D, _ptr(dw), _ptr(db), _ptr(seq_off), _ptr(state), rows, S, D, W, code, flags, _ptr(sc), nbytes)
         return dx, dw, db, None, None, None, None, None, None
 
 
@@ -350,7 +361,7 @@ def causal_conv(x, weight, bias=None, *, silu=False, seq_off=None, state=None, r
     on the row itself), bias [D].  `state` [S, W-1, D] in x's type holds the inputs in front of every sequence (oldest
     first; zeros without it) and carries no gradient; with `return_state` the call gives (y, state behind the end)."""
     what = 'causal_conv'
-    _first(what, x, (2, 3))
+    _first(what, x, 2, 3)
     rows, S = _sequences(what, x, seq_off)
     weight, bias = _conv_params(what, x, weight, bias)
     if state is not None:
@@ -370,7 +381,7 @@ def causal_conv_step(x, state, weight, bias=None, *, silu=False, state_out=None)
     """One row x [S, D] for each of S sequences.  `state` [S, W-1, D] is moved on by the row, in place or into
     `state_out`; returns (y, the new state).  No gradients."""
     what = 'causal_conv_step'
-    _first(what, x, (2,))
+    _first(what, x, 2, 2)
     S, D = x.shape
     weight, bias = _conv_params(what, x, weight, bias)
     if _wants_grad(x, state, weight, bias):
@@ -398,30 +409,35 @@ def _state_out(what, state, out):
     return out
 
 
-def _scan_struct(x, ldx, dt, lddt, A, B, ldb, C, ldc, D, z, ldz, bias, h0, seq_off, rows, S, G, flags):
+def _scan_call(x, dt, A, B, C, D, z, bias, h0, seq_off, ld, rows, S, G, flags):
+    """The operands as the library takes them; ld: the row distances of x, dt, B, C and z."""
     width, N = A.shape
-    return _lib.Scan(_ptr(x), _ptr(dt), _ptr(B), _ptr(C), _ptr(z), ldx, lddt, ldb, ldc, ldz, _ptr(A), _ptr(D), _ptr(bias), _ptr(h0), _ptr(seq_off),
-                     rows, S, width, G, N, _DTYPES[x.dtype], flags)
+    return _lib.Scan(x.data_ptr(), dt.data_ptr(), B.data_ptr(), C.data_ptr(), _ptr(z), *ld, A.data_ptr(), _ptr(D), _ptr(bias), _ptr(h0),
+                     _ptr(seq_off), rows, S, width, G, N, _DTYPES[x.dtype], flags)
 
 
-def _scan_rows(x, dt, B, C, z, width, G, N):
-    """The activation operands as rows, with their distances, in psvae_scan's order: x, dt, (A), B, C, (skip), z."""
-    return [_rows(x, width), _rows(dt, width), _rows(B, G * N), _rows(C, G * N), (None, 0) if z is None else _rows(z, width)]
+def _scan_rows(x, dt, B, C, z, width, gn):
+    """The activation operands as rows, and their distances."""
+    x, ldx = _rows(x, width)
+    dt, lddt = _rows(dt, width)
+    B, ldb = _rows(B, gn)
+    C, ldc = _rows(C, gn)
+    z, ldz = (None, 0) if z is None else _rows(z, width)
+    return x, dt, B, C, z, (ldx, lddt, ldb, ldc, ldz)
 
 
 def _scan_forward(x, dt, A, B, C, D, z, bias, h0, seq_off, flags, rows, S, G, want_state, keep):
     L = _lib.lib()
     (width, N), dev = A.shape, x.device
-    ops2 = _scan_rows(x, dt, B, C, z, width, G, N)
-    (x2, ldx), (dt2, lddt), (B2, ldb), (C2, ldc), (z2, ldz) = ops2
-    a = _scan_struct(x2, ldx, dt2, lddt, A, B2, ldb, C2, ldc, D, z2, ldz, bias, h0, seq_off, rows, S, G, flags)
+    x2, dt2, B2, C2, z2, ld = _scan_rows(x, dt, B, C, z, width, G * N)
+    a = _scan_call(x2, dt2, A, B2, C2, D, z2, bias, h0, seq_off, ld, rows, S, G, flags)
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
     last = torch.empty(S, width, N, dtype=torch.float32, device=dev) if want_state else None
-    kept = _scratch(L.psvae_selective_scan_saved_bytes(rows, S, width, G, N), dev) if keep else None
+    kept = torch.empty(L.psvae_selective_scan_saved_bytes(rows, S, width, G, N), dtype=torch.uint8, device=dev) if keep else None
     nbytes = L.psvae_selective_scan_scratch_bytes(rows, S, width, G, N, 0)
-    sc = _scratch(nbytes, dev) if nbytes else None
+    sc = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _run('psvae_selective_scan_forward', dev, L.psvae_selective_scan_forward, a, y.data_ptr(), width, _ptr(last), _ptr(kept), _ptr(sc), nbytes)
-    return y, last, kept, ops2
+    return y, last, kept, (x2, dt2, B2, C2, z2, ld)
 
 
 class SelectiveScanFn(torch.autograd.Function):
@@ -429,40 +445,37 @@ class SelectiveScanFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, dt, A, B, C, D, z, bias, h0, seq_off, flags, rows, S, G, want_state):
-        y, last, kept, ops2 = _scan_forward(x, dt, A, B, C, D, z, bias, h0, seq_off, flags, rows, S, G, want_state, True)
-        (x2, _), (dt2, _), (B2, _), (C2, _), (z2, _) = ops2
+        y, last, kept, (x2, dt2, B2, C2, z2, ld) = _scan_forward(x, dt, A, B, C, D, z, bias, h0, seq_off, flags, rows, S, G, want_state, True)
         ctx.save_for_backward(x2, dt2, A, B2, C2, D, z2, bias, seq_off, kept)
-        ctx.ld = [ld for _, ld in ops2]
-        ctx.call = flags, rows, S, G
-        ctx.shapes = x.shape, B.shape, C.shape, None if h0 is None else h0.shape
+        ctx.call = ld, flags, rows, S, G, x.shape, B.shape
         ctx.set_materialize_grads(False)
         return y, last
 
     @staticmethod
     @_once
     def backward(ctx, dy, dlast):
-        L = _lib.lib()
+        L, empty, f32 = _lib.lib(), torch.empty, torch.float32
         x, dt, A, B, C, D, z, bias, seq_off, kept = ctx.saved_tensors
-        flags, rows, S, G = ctx.call
-        xs, bs, cs, hs = ctx.shapes
-        ldx, lddt, ldb, ldc, ldz = ctx.ld
-        (width, N), dev = A.shape, x.device
-        dy = torch.zeros(xs, dtype=x.dtype, device=dev) if dy is None else dy
+        ld, flags, rows, S, G, shape, bc_shape = ctx.call
+        (width, N), dev, dtype = A.shape, A.device, x.dtype
+        if dy is None:
+            dy = torch.zeros(shape, dtype=dtype, device=dev)
         dy2, lddy = _rows(dy, width)
-        dlast = None if dlast is None else _f32c(dlast)
-        a = _scan_struct(x, ldx, dt, lddt, A, B, ldb, C, ldc, D, z, ldz, bias, None, seq_off, rows, S, G, flags)
-
-        def like(shape, dtype=x.dtype):
-            return torch.empty(shape, dtype=dtype, device=dev)
-        f32 = torch.float32
-        dx, ddt, dB, dC, dz = like(xs), like(xs), like(bs), like(cs), None if z is None else like(xs)
-        dA, dD = like((width, N), f32), None if D is None else like(width, f32)
-        dbias, dh0 = None if bias is None else like(width, f32), None if hs is None else like(hs, f32)
-        g = _lib.ScanGrads(_ptr(dx), _ptr(ddt), _ptr(dB), _ptr(dC), _ptr(dz), _ptr(dA), _ptr(dD), _ptr(dbias), _ptr(dh0))
+        if dlast is not None:
+            dlast = _f32c(dlast)
+        a = _scan_call(x, dt, A, B, C, D, z, bias, None, seq_off, ld, rows, S, G, flags)
+        dx, ddt = empty(shape, dtype=dtype, device=dev), empty(shape, dtype=dtype, device=dev)
+        dB, dC = empty(bc_shape, dtype=dtype, device=dev), empty(bc_shape, dtype=dtype, device=dev)
+        dz = None if z is None else empty(shape, dtype=dtype, device=dev)
+        dA = empty(width, N, dtype=f32, device=dev)
+        dD = None if D is None else empty(width, dtype=f32, device=dev)
+        dbias = None if bias is None else empty(width, dtype=f32, device=dev)
+        dh0 = empty(S, width, N, dtype=f32, device=dev) if ctx.needs_input_grad[8] else None
+        g = _lib.ScanGrads(dx.data_ptr(), ddt.data_ptr(), dB.data_ptr(), dC.data_ptr(), _ptr(dz), dA.data_ptr(), _ptr(dD), _ptr(dbias), _ptr(dh0))
         nbytes = L.psvae_selective_scan_scratch_bytes(rows, S, width, G, N, 1)
-        sc = _scratch(nbytes, dev)
-        _run('psvae_selective_scan_backward', dev, L.psvae_selective_scan_backward, a, _ptr(kept), dy2.data_ptr(), lddy, _ptr(dlast), g, sc.data_ptr(),
-             sc.numel())
+        sc = empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+        _run('psvae_selective_scan_backward', dev, L.psvae_selective_scan_backward, a, kept.data_ptr(), dy2.data_ptr(), lddy, _ptr(dlast), g,
+             sc.data_ptr(), nbytes)
         return dx, ddt, dA, dB, dC, dD, dz, dbias, dh0, None, None, None, None, None, None
 
 
@@ -495,7 +508,7 @@ def selective_scan(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, softplus=Tru
     with up to 64 states; D, dt_bias [width]; h0 [S, width, N], the state in front of every sequence (zeros without
     it).  Returns y, with `return_state` (y, the state behind every sequence's end), which carries gradients."""
     what = 'selective_scan'
-    _first(what, x, (2, 3))
+    _first(what, x, 2, 3)
     rows, S = _sequences(what, x, seq_off)
     A, D, dt_bias, h0, G = _scan_operands(what, x, dt, A, B, C, D, z, dt_bias, h0, S)
     flags = (_lib.SEQ_SOFTPLUS if softplus else 0) | (_lib.SEQ_ZERO_OUTSIDE if seq_off is not None else 0)
@@ -510,7 +523,7 @@ def selective_scan_step(x, dt, A, B, C, state, *, D=None, z=None, dt_bias=None, 
     """One row of the scan for each of S sequences: x, dt, z [S, width], B, C [S, N] or [S, G, N].  `state` [S, width, N]
     fp32 is moved on, in place or into `state_out`; returns (y, the new state).  No gradients."""
     what = 'selective_scan_step'
-    _first(what, x, (2,))
+    _first(what, x, 2, 2)
     S, width = x.shape
     if state.dtype != torch.float32:
         raise ValueError(f'{what}: state is {state.dtype}, expected torch.float32')
@@ -518,8 +531,8 @@ def selective_scan_step(x, dt, A, B, C, state, *, D=None, z=None, dt_bias=None, 
         raise RuntimeError(f'{what} has no backward pass: call it under torch.no_grad() or on detached tensors')
     out = _state_out(what, state, state_out)
     A, D, dt_bias, state, G = _scan_operands(what, x, dt, A, B, C, D, z, dt_bias, state, S)
-    (x2, ldx), (dt2, lddt), (B2, ldb), (C2, ldc), (z2, ldz) = _scan_rows(x, dt, B, C, z, width, G, A.shape[1])
-    a = _scan_struct(x2, ldx, dt2, lddt, A, B2, ldb, C2, ldc, D, z2, ldz, dt_bias, state, None, S, S, G, _lib.SEQ_SOFTPLUS if softplus else 0)
+    x2, dt2, B2, C2, z2, ld = _scan_rows(x, dt, B, C, z, width, G * A.shape[1])
+    a = _scan_call(x2, dt2, A, B2, C2, D, z2, dt_bias, state, None, ld, S, S, G, _lib.SEQ_SOFTPLUS if softplus else 0)
     y = torch.empty(S, width, dtype=x.dtype, device=x.device)
     _run('psvae_selective_scan_step', x.device, _lib.lib().psvae_selective_scan_step, a, y.data_ptr(), width, out.data_ptr())
     return y, out
