@@ -125,31 +125,19 @@ __device__ __forceinline__ int64_t kept_row(int begin, int s, int tile) { return
 // that the 16 lanes that write one row of 64 (or 32) channels reach as many bank groups.
 __device__ __forceinline__ int quarter(int q, int ch) { return 4 * (q ^ (ch >> 4 & 3)); }
 
-// V elements of a row, zeros from the n-th on.  `base` is the same for the workgroup, the lane's distance from it fits 32
-// bits (rows lie less than 2^26 elements apart).
-template <bool VEC, class T, int V>
-__device__ __forceinline__ void fetch_row(const void* base, unsigned offset, int n, Raw<T, V>& out) {
-    asm volatile("" : "+v"(offset));       // keeps base + offset in the instruction: hoisted sums would fill the registers
-    const T* p = (const T*)((const char*)base + offset);
-    if constexpr (V == 1) {
-        out.v[0] = (T)0.f;
-        if (n > 0) out.v[0] = p[0];
+// V elements of a row, zeros from the n-th on.
+template <bool VEC, class T, int V> __device__ __forceinline__ void fetch_row(const T* p, int n, Raw<T, V>& out) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out.v[i] = (T)0.f;
+    if constexpr (VEC) {
+        if (n > 0) out.load(p);
     } else {
-        typename VecOf<T, V>::type q = (T)0.f;
-        if constexpr (VEC) {
-            if (n > 0) q = *(const typename VecOf<T, V>::type*)p;
-        } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (i < n) q[i] = p[i];
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) out.v[i] = q[i];
+        for (int i = 0; i < V; ++i)
+            if (i < n) out.v[i] = p[i];
     }
 }
-template <bool VEC, class T, int V> __device__ __forceinline__ void store_row(void* base, unsigned offset, int n, const float (&in)[V]) {
-    asm volatile("" : "+v"(offset));
-    T* p = (T*)((char*)base + offset);
+template <bool VEC, class T, int V> __device__ __forceinline__ void store_row(T* p, int n, const float (&in)[V]) {
     if constexpr (VEC) {
         if (n > 0) store_vec<V>(p, in);
     } else {
@@ -158,31 +146,20 @@ template <bool VEC, class T, int V> __device__ __forceinline__ void store_row(vo
             if (i < n) p[i] = (T)in[i];
     }
 }
-// The rows of one operand as a workgroup reads or writes them: the tile's first row (uniform) and the lane's place in it.
-struct RowsOf {
-    char* base; int64_t step; unsigned offset;       // step: bytes from one tile to the next
-    __device__ __forceinline__ RowsOf(const void* p, int64_t ld, int unit, int64_t row, int col, int r, int c)
-        : base((char*)p + (row * ld + col) * unit), step(ld * unit * TILE), offset((unsigned)(r * ld + c) * unit) {}
-};
 
-// A tile's B or C, element by element (fewer than the rows' own elements by the channels over the states).
-template <class T, int P, int K> struct TileBC {
-    static constexpr int NP = P * K, COUNT = Shape<P, K>::NBC;
-    T v[COUNT];
-    __device__ __forceinline__ void fetch(const char* base, int64_t ld, int N, int rows) {
+// A tile's B or C: a lane has NBC states of one row (with 8 or 4 states some lanes have none).
+template <class T, int P, int K, bool VEC> struct TileBC {
+    static constexpr int NP = P * K, V = Shape<P, K>::NBC;
+    Raw<T, V> v;
+    static __device__ __forceinline__ int row() { return threadIdx.x * V / NP; }
+    static __device__ __forceinline__ int state() { return threadIdx.x * V % NP; }
+    __device__ __forceinline__ void fetch(const T* p, int N, int rows) { fetch_row<VEC>(p, row() < rows ? N - state() : 0, v); }   // p: the lane's place
+    __device__ __forceinline__ void put(float* tile) const {
+        if (TILE * NP < 256 && (int)threadIdx.x >= TILE * NP) return;
+        float f[V];
 #pragma unroll
-        for (int j = 0; j < COUNT; ++j) {
-            const int e = j * 256 + threadIdx.x, r = e / NP, n = e % NP;
-            v[j] = (T)0.f;
-            unsigned at = (unsigned)(r * ld + n) * (unsigned)sizeof(T);
-            asm volatile("" : "+v"(at));
-            if (r < rows && n < N) v[j] = *(const T*)(base + at);
-        }
-    }
-    __device__ __forceinline__ void put(float* lds) const {            // lds: the workgroup's tile + threadIdx.x
-#pragma unroll
-        for (int j = 0; j < COUNT; ++j)
-            if (j * 256 + 255 < TILE * NP || j * 256 + (int)threadIdx.x < TILE * NP) lds[j * 256] = (float)v[j];
+        for (int i = 0; i < V; ++i) f[i] = v[i];
+        store_vec<V>(tile + threadIdx.x * V, f);
     }
 };
 
@@ -257,22 +234,22 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Scan q) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) h[k] = fmaf(__builtin_amdgcn_exp2f(ds * A2[k]), h[k], e[k]);
             }
-        const int64_t first = sq.begin + (int64_t)tiles.first * TILE;
-        RowsOf rx(q.x, q.ldx, U, first, w.c0, r, c), rt(q.dt, q.lddt, U, first, w.c0, r, c), rz(q.z, q.ldz, U, first, w.c0, r, c),
-            ry(q.y, q.ldy, U, first, w.c0, r, c);
-        const char *pb = (const char*)q.B + (first * q.ldb + w.g * q.N) * U, *pc = (const char*)q.C + (first * q.ldc + w.g * q.N) * U;
+        const int64_t first = sq.begin + (int64_t)tiles.first * TILE, row = first + r, bc_row = first + TileBC<T, P, K, VEC>::row();
+        const T *px = (const T*)q.x + row * q.ldx + w.c0 + c, *pt = (const T*)q.dt + row * q.lddt + w.c0 + c,
+                *pz = (const T*)q.z + row * q.ldz + w.c0 + c, *pb = (const T*)q.B + bc_row * q.ldb + w.g * q.N + TileBC<T, P, K, VEC>::state(),
+                *pc = (const T*)q.C + bc_row * q.ldc + w.g * q.N + TileBC<T, P, K, VEC>::state();
+        T* py = (T*)q.y + row * q.ldy + w.c0 + c;
         float* keep = q.kept ? own_state<K>(q.kept, kept_row(sq.begin, s, tiles.first), q, NP, d, n0) : nullptr;
         Raw<T, VE> nx, nt, nz;
-        TileBC<T, P, K> nb, nc;
+        TileBC<T, P, K, VEC> nb, nc;
         auto fetch = [&](int rows) {
             const int n = r < rows ? left : 0;
-            fetch_row<VEC>(rx.base, rx.offset, n, nx);
-            fetch_row<VEC>(rt.base, rt.offset, n, nt);
-            if (gated) fetch_row<VEC>(rz.base, rz.offset, n, nz);
-            nb.fetch(pb, q.ldb, q.N, rows);
-            if (!ENDS) nc.fetch(pc, q.ldc, q.N, rows);
-            rx.base += rx.step; rt.base += rt.step; rz.base += rz.step;
-            pb += q.ldb * (U * TILE); pc += q.ldc * (U * TILE);
+            fetch_row<VEC>(px, n, nx);
+            fetch_row<VEC>(pt, n, nt);
+            if (gated) fetch_row<VEC>(pz, n, nz);
+            nb.fetch(pb, q.N, rows);
+            if (!ENDS) nc.fetch(pc, q.N, rows);
+            px += TILE * q.ldx; pt += TILE * q.lddt; pz += TILE * q.ldz; pb += TILE * q.ldb; pc += TILE * q.ldc;
         };
         int remain = sq.end - (int)first;               // rows from this tile's first to the sequence's end
         if (tiles.first < tiles.last) fetch(min(TILE, remain));
@@ -289,8 +266,8 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Scan q) {
                 at_row[DELTA + i * PITCH] = v;
                 at_row[DX + i * PITCH] = v * cx[i];
             }
-            nb.put(lds + BT + threadIdx.x);
-            if (!ENDS) nc.put(lds + CT + threadIdx.x);
+            nb.put(lds + BT);
+            if (!ENDS) nc.put(lds + CT);
             __syncthreads();
             if (tile + 1 < tiles.last) fetch(min(TILE, remain - TILE));
 #pragma unroll
@@ -329,8 +306,8 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Scan q) {
                     o[i] = fmaf(skip[i], cx[i], at_row[YT + i * PITCH]);
                     if (gated) o[i] *= cz[i] * sigmoidf(cz[i]);
                 }
-                store_row<VEC, T, VE>(ry.base, ry.offset, n, o);
-                ry.base += ry.step;
+                store_row<VEC>(py, n, o);
+                py += TILE * q.ldy;
             }
         }
         if (ENDS) {
@@ -342,7 +319,6 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Scan q) {
         } else if (q.hT && chunk == q.chunks - 1 && live) {
             save_state<K>(q.hT, s, q, d, n0, h);
         }
-        __syncthreads();                               // the last tile's y is read before the next sequence writes it
     }
 }
 
@@ -399,43 +375,47 @@ __global__ __launch_bounds__(256, CARRY ? 4 : 2) void scan_bwd_kernel(Scan q) {
                 for (int k = 0; k < K; ++k) ag[k] = fmaf(__builtin_amdgcn_exp2f(ds * A2[k]), ag[k], e[k]);
             }
         const int64_t first = sq.begin + (int64_t)(tiles.last - 1) * TILE;     // the last tile's first row
-        RowsOf rx(q.x, q.ldx, U, first, w.c0, r, c), rt(q.dt, q.lddt, U, first, w.c0, r, c), rz(q.z, q.ldz, U, first, w.c0, r, c),
-            rg(q.dy, q.lddy, U, first, w.c0, r, c);
-        const unsigned out = (unsigned)(r * q.Dn + c) * U;
-        int64_t out0 = (first * q.Dn + w.c0) * U;      // the gradients are contiguous
-        const char *pb = (const char*)q.B + (first * q.ldb + w.g * q.N) * U, *pc = (const char*)q.C + (first * q.ldc + w.g * q.N) * U;
+        const int64_t row = first + r, bc_row = first + TileBC<T, P, K, VEC>::row();
+        const T *px = (const T*)q.x + row * q.ldx + w.c0 + c, *pt = (const T*)q.dt + row * q.lddt + w.c0 + c,
+                *pz = (const T*)q.z + row * q.ldz + w.c0 + c, *pg = (const T*)q.dy + row * q.lddy + w.c0 + c,
+                *pb = (const T*)q.B + bc_row * q.ldb + w.g * q.N + TileBC<T, P, K, VEC>::state(),
+                *pc = (const T*)q.C + bc_row * q.ldc + w.g * q.N + TileBC<T, P, K, VEC>::state();
+        int64_t out = row * q.Dn + w.c0 + c;           // the gradients are contiguous
         const float* keep = CARRY ? nullptr : own_state<K>(q.kept, kept_row(sq.begin, s, tiles.last - 1), q, NP, d, n0);
         float* bc_out = CARRY ? nullptr : q.part_bc + (((int64_t)w.blk * q.T + first) * q.G + w.g) * 2 * NP;
         Raw<T, VE> nx, nt, nz, ng;
-        TileBC<T, P, K> nb, nc;
+        TileBC<T, P, K, VEC> nb, nc;
         float nh[TILE / HALF][K];
         auto fetch = [&](int rows) {
             const int n = r < rows ? left : 0;
-            fetch_row<VEC>(rt.base, rt.offset, n, nt);
-            fetch_row<VEC>(rg.base, rg.offset, n, ng);
-            if (gated) fetch_row<VEC>(rz.base, rz.offset, n, nz);
-            nc.fetch(pc, q.ldc, q.N, rows);
-            rt.base -= rt.step; rg.base -= rg.step; rz.base -= rz.step;
-            pc -= q.ldc * (U * TILE);
+            fetch_row<VEC>(pt, n, nt);
+            fetch_row<VEC>(pg, n, ng);
+            if (gated) fetch_row<VEC>(pz, n, nz);
+            nc.fetch(pc, q.N, rows);
             if constexpr (!CARRY) {
-                fetch_row<VEC>(rx.base, rx.offset, n, nx);
-                nb.fetch(pb, q.ldb, q.N, rows);
+                fetch_row<VEC>(px, n, nx);
+                nb.fetch(pb, q.N, rows);
 #pragma unroll
-                for (int half = 0; half < TILE / HALF; ++half)
+                for (int half = 0; half < TILE / HALF; ++half) {
 #pragma unroll
-                    for (int k = 0; k < K; ++k) nh[half][k] = live && half * HALF < rows ? keep[(int64_t)half * q.Dn * NP + k] : 0.f;
-                rx.base -= rx.step;
-                pb -= q.ldb * (U * TILE);
+                    for (int k = 0; k < K; ++k) nh[half][k] = 0.f;
+                    if (live && half * HALF < rows)
+#pragma unroll
+                        for (int k = 0; k < K; ++k) nh[half][k] = keep[(int64_t)half * q.Dn * NP + k];
+                }
+            }
+            pt -= TILE * q.lddt; pg -= TILE * q.lddy; pz -= TILE * q.ldz; pc -= TILE * q.ldc;
+            if constexpr (!CARRY) {
+                px -= TILE * q.ldx;
+                pb -= TILE * q.ldb;
                 keep -= (int64_t)q.Dn * NP * (TILE / HALF);
             }
         };
-        int rows = sq.end - (int)first;                 // the last tile of the sequence may be short
-        rows = min(rows, TILE);
-        if (tiles.first < tiles.last) fetch(rows);
-        for (int tile = tiles.last - 1; tile >= tiles.first; --tile, rows = TILE) {
+        Raw<T, VE> cx, cz, cg;
+        float h[TILE / HALF][K];
+        auto stage = [&](int rows) {
             const int n = r < rows ? left : 0;
-            Raw<T, VE> cx = nx, cz = nz, cg = ng;
-            float h[TILE / HALF][K];
+            cx = nx; cz = nz; cg = ng;
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
                 float v = (float)nt.v[i] + s_bias[c + i], dy = (float)cg.v[i], slope = 1.f;
@@ -446,12 +426,21 @@ __global__ __launch_bounds__(256, CARRY ? 4 : 2) void scan_bwd_kernel(Scan q) {
                 at_row[DY + i * PITCH] = dy;
                 if constexpr (!CARRY) { at_row[DX + i * PITCH] = v * (float)cx.v[i]; at_row[SLOPE + i * PITCH] = slope; }
             }
-            if constexpr (!CARRY) nb.put(lds + BT + threadIdx.x);
-            nc.put(lds + CT + threadIdx.x);
+            if constexpr (!CARRY) nb.put(lds + BT);
+            nc.put(lds + CT);
 #pragma unroll
             for (int half = 0; half < TILE / HALF; ++half)
 #pragma unroll
                 for (int k = 0; k < K; ++k) h[half][k] = nh[half][k];
+        };
+        int rows = sq.end - (int)first;                 // the last tile of the sequence may be short
+        rows = min(rows, TILE);
+        if (tiles.first < tiles.last) {
+            fetch(rows);
+            stage(rows);
+        }
+        for (int tile = tiles.last - 1; tile >= tiles.first; --tile, rows = TILE) {
+            const int n = r < rows ? left : 0;
             __syncthreads();
             if (tile > tiles.first) fetch(TILE);
             if constexpr (CARRY) {
@@ -474,6 +463,7 @@ __global__ __launch_bounds__(256, CARRY ? 4 : 2) void scan_bwd_kernel(Scan q) {
                     }
                 }
                 __syncthreads();
+                if (tile > tiles.first) stage(TILE);
             } else {
                 float dAt[K];
 #pragma unroll
@@ -572,15 +562,26 @@ __global__ __launch_bounds__(256, CARRY ? 4 : 2) void scan_bwd_kernel(Scan q) {
                     dD[i] = fmaf(dyp, x, dD[i]);
                     dbias[i] += odt[i];
                 }
-                store_row<VEC, T, VE>((char*)q.dx + out0, out, n, odx);
-                store_row<VEC, T, VE>((char*)q.ddt + out0, out, n, odt);
-                if (gated) store_row<VEC, T, VE>((char*)q.dz + out0, out, n, odz);
-                out0 -= (int64_t)q.Dn * U * TILE;
-                for (int i = threadIdx.x; i < rows * 2 * NP; i += 256)
-                    bc_out[(int64_t)(i / (2 * NP)) * q.G * 2 * NP + i % (2 * NP)] =
-                        (lds[BC + i] + lds[BC + BCW + i]) + (lds[BC + 2 * BCW + i] + lds[BC + 3 * BCW + i]);
-                bc_out -= (int64_t)q.G * 2 * NP * TILE;
+                constexpr int BCN = (BCW + 255) / 256;
+                float bc[BCN];
+#pragma unroll
+                for (int j = 0; j < BCN; ++j) {
+                    const float* p = lds + BC + j * 256 + threadIdx.x;
+                    bc[j] = j * 256 + 255 < BCW || j * 256 + (int)threadIdx.x < BCW ? (p[0] + p[BCW]) + (p[2 * BCW] + p[3 * BCW]) : 0.f;
+                }
                 __syncthreads();
+                // the next tile first: a wait for its rows behind these stores would be one for the stores, too
+                if (tile > tiles.first) stage(TILE);
+                store_row<VEC>((T*)q.dx + out, n, odx);
+                store_row<VEC>((T*)q.ddt + out, n, odt);
+                if (gated) store_row<VEC>((T*)q.dz + out, n, odz);
+                out -= (int64_t)TILE * q.Dn;
+#pragma unroll
+                for (int j = 0; j < BCN; ++j) {
+                    const int e = j * 256 + threadIdx.x;
+                    if (e < rows * 2 * NP) bc_out[(int64_t)(e / (2 * NP)) * q.G * 2 * NP + e % (2 * NP)] = bc[j];
+                }
+                bc_out -= (int64_t)q.G * 2 * NP * TILE;
             }
         }
         if (CARRY) {
@@ -776,7 +777,9 @@ Scan scan_args(const psvae_scan* a, const Plan& p) {
     q.T = (int)a->T; q.S = a->S; q.Dn = a->D; q.G = a->G; q.N = a->N; q.chunks = p.chunks;
     q.softplus = (a->flags & PSVAE_SEQ_SOFTPLUS) != 0;
     q.zero_outside = a->seq_off && (a->flags & PSVAE_SEQ_ZERO_OUTSIDE);
-    q.vec = a->D / a->G % p.VE == 0 && rows_vec(a->x, a->ldx, p.VE, a->dtype) && rows_vec(a->dt, a->lddt, p.VE, a->dtype) &&
+    const int bc = p.NP > 16 ? p.NP / 16 : 1;          // B and C are read NBC states at a time
+    q.vec = a->N % bc == 0 && rows_vec(a->B, a->ldb, bc, a->dtype) && rows_vec(a->C, a->ldc, bc, a->dtype) &&
+            a->D / a->G % p.VE == 0 && rows_vec(a->x, a->ldx, p.VE, a->dtype) && rows_vec(a->dt, a->lddt, p.VE, a->dtype) &&
             rows_vec(a->z, a->ldz, p.VE, a->dtype);
     return q;
 }
