@@ -733,11 +733,21 @@ Plan scan_plan(int64_t T, int S, int D, int G, int N) {
     p.VE = p.CB >= 64 ? 4 : p.CB / 16;
     p.tiles = (D / G + p.CB - 1) / p.CB;
     p.blocks = p.tiles * G;
-    // Chunks: the two-pass form computes every exponential twice, so it is taken only where workgroups of whole sequences
-    // leave more than half of the chip idle (fewer than two for every CU), and a chunk has four tiles at least on average.
+    // Chunks: the two-pass form computes every exponential twice, so it is taken only where workgroups of whole sequences are
+    // fewer than two for every CU (16 x 1024 x 2048, 16 states: 512 workgroups in one piece 174 + 480 us forward + backward,
+    // in two 205 + 537; 12 x 1365: 384 in one piece 229 + 631, in four 227 + 554).  Then there are four for every CU at least,
+    // as near above a whole number of them as 5 % where twice as many pieces reach that (12 x 1365: three pieces make 4.5 for
+    // every CU and take 233 + 593), and a piece has four tiles on average.
     const int64_t whole = (int64_t)p.blocks * (S > 0 ? S : 1), tiles = (T + TILE - 1) / TILE;
     int64_t c = 1;
-    if (whole < 512) c = (1024 + whole - 1) / whole;
+    if (whole < 512) {
+        const int64_t least = (1024 + whole - 1) / whole;
+        double best = 2.;
+        for (int64_t i = least; i <= 2 * least && best > 1.05; ++i) {
+            const double each = (double)(whole * i) / 256, idle = (double)((whole * i + 255) / 256) / each;
+            if (idle < best) { best = idle; c = i; }
+        }
+    }
     const int64_t most = tiles / (4 * (int64_t)(S > 0 ? S : 1));
     if (c > most) c = most;
     if (opt(OPT_SCAN_CHUNKS) >= 1) c = opt(OPT_SCAN_CHUNKS);
