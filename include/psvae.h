@@ -498,12 +498,13 @@ int psvae_causal_conv_step(const void* x, int64_t ldx, const void* state, void* 
  *   h[t, d, n] = exp(delta[t, d] A[d, n]) h[t-1, d, n] + delta[t, d] x[t, d] B[t, g, n]
  *   y[t, d] = (sum_n C[t, g, n] h[t, d, n] + skip[d] x[t, d]) * silu(z[t, d])
  * x, dt, z [T, D], B and C [T, G N] of `dtype`; A [D, N], skip [D], dt_bias [D] and the states h0, hT [S, D, N] fp32,
- * contiguous; leading dimensions below 2^26.  z, skip, dt_bias, h0 (and, as outputs, hT) may be NULL.
- * _forward: with `saved` (psvae_selective_scan_saved_bytes, 16-byte aligned; the state every 16 rows) a backward pass can
- *   follow.  scratch: psvae_selective_scan_scratch_bytes(.., backward = 0), 0 where the time axis is not cut.
+ * contiguous.  z, skip, dt_bias, h0 (and, as outputs, hT) may be NULL.
+ * _forward: with `saved` (psvae_selective_scan_saved_bytes, 16-byte aligned: the state every 8 rows, 4 D N / 8 bytes a row)
+ *   a backward pass can follow.  scratch: psvae_selective_scan_scratch_bytes(.., backward = 0), 0 where the time axis is not cut.
  * _backward: given dy (gradient of y) and dhT (of hT, or NULL), writes every gradient of psvae_scan_grads; dz may be NULL
  *   without z, and d_skip, d_dt_bias and dh0 where they are not wanted.  Same `a` and `saved` as the forward call.
- *   scratch: psvae_selective_scan_scratch_bytes(.., backward = 1), 16-byte aligned.
+ *   scratch: psvae_selective_scan_scratch_bytes(.., backward = 1), 16-byte aligned; most of it holds sums for dB and dC,
+ *   8 N bytes a row for every 64 channels (32 with more than 16 states, 16 with more than 32).
  * _step: one row for each of S sequences (T = S, no seq_off): reads h0, writes hT, which may be h0. */
 typedef struct psvae_scan {
     const void *x, *dt, *B, *C, *z;

@@ -163,6 +163,15 @@ template <class T, int P, int K, bool VEC> struct TileBC {
     }
 };
 
+// A log2 e, kept finite: rows behind a sequence's end have delta = 0, and 0 x infinity would not leave their states alone.
+template <int K> __device__ __forceinline__ void scale_rates(float (&A)[K]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        A[k] *= LOG2E;
+        A[k] = A[k] < -3e38f ? -3e38f : (A[k] > 3e38f ? 3e38f : A[k]);
+    }
+}
+
 // State of (channel d, states p K ..) in an array [rows][D][N]; lanes past the states read 0 and write nothing.
 template <int K> __device__ __forceinline__ void load_state(const float* base, int64_t row, const Scan& q, int d, int n0, float (&h)[K]) {
 #pragma unroll
@@ -214,8 +223,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Scan q) {
     const bool live = ch < w.nc, gated = !ENDS && q.z;
     float A2[K], bias[VE], skip[VE];
     load_state<K>(live ? q.A : nullptr, 0, q, d, n0, A2);
-#pragma unroll
-    for (int k = 0; k < K; ++k) A2[k] *= LOG2E;
+    scale_rates<K>(A2);
 #pragma unroll
     for (int i = 0; i < VE; ++i) {
         bias[i] = q.bias && i < left ? q.bias[w.c0 + c + i] : 0.f;
@@ -352,8 +360,9 @@ __global__ __launch_bounds__(256, CARRY ? 4 : 2) void scan_bwd_kernel(Scan q) {
     const bool live = ch < w.nc, gated = q.z;          // lanes without a channel compute with zeros
     float A2[K], dA[K], dD[VE], dbias[VE];
     load_state<K>(live ? q.A : nullptr, 0, q, d, n0, A2);
+    scale_rates<K>(A2);
 #pragma unroll
-    for (int k = 0; k < K; ++k) { A2[k] *= LOG2E; dA[k] = 0.f; }
+    for (int k = 0; k < K; ++k) dA[k] = 0.f;
 #pragma unroll
     for (int i = 0; i < VE; ++i) dD[i] = dbias[i] = 0.f;
     for (int i = threadIdx.x; i < Sh::CB; i += 256) {
@@ -698,6 +707,7 @@ template <class T, int P, int K, int R> __global__ __launch_bounds__(256) void s
     }
     if (vec_state) load_vec<K>(q.A + (int64_t)d * q.N + n0, A);
     else load_state<K>(q.A, 0, q, d, n0, A);
+    scale_rates<K>(A);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int s = s0 + i;
@@ -706,7 +716,7 @@ template <class T, int P, int K, int R> __global__ __launch_bounds__(256) void s
         if (q.softplus) delta = softplus_slope(v[i], slope);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            h[i][k] = fmaf(__builtin_amdgcn_exp2f(delta * (A[k] * LOG2E)), h[i][k], delta * x[i] * b[i][k]);
+            h[i][k] = fmaf(__builtin_amdgcn_exp2f(delta * A[k]), h[i][k], delta * x[i] * b[i][k]);
             if (n0 + k < q.N) y = fmaf(h[i][k], c[i][k], y);
         }
         y = lanes_add<P>(y);
@@ -773,8 +783,6 @@ int scan_operands(const psvae_scan* a) {
     if (a->flags & ~(PSVAE_SEQ_SOFTPLUS | PSVAE_SEQ_ZERO_OUTSIDE)) return PSVAE_E_SHAPE;
     if (a->T > 0 && (!a->x || !a->dt || !a->B || !a->C)) return PSVAE_E_NULL;
     if (!a->A) return PSVAE_E_NULL;
-    constexpr int64_t FAR = 1 << 26;       // a tile's rows lie within 32-bit distances
-    if (a->ldx >= FAR || a->lddt >= FAR || a->ldb >= FAR || a->ldc >= FAR || (a->z && a->ldz >= FAR)) return PSVAE_E_SHAPE;
     if (a->ldx < a->D || a->lddt < a->D || a->ldb < (int64_t)a->G * a->N || a->ldc < (int64_t)a->G * a->N || (a->z && a->ldz < a->D)) return PSVAE_E_SHAPE;
     return 0;
 }
@@ -870,7 +878,7 @@ extern "C" size_t psvae_selective_scan_saved_bytes(int64_t T, int S, int D, int 
 extern "C" int psvae_selective_scan_forward(const psvae_scan* a, void* y, int64_t ldy, float* hT, void* saved, void* scratch,
                                             size_t scratch_bytes, void* stream) {
     PSVAE_TRY(scan_operands(a));
-    if (ldy < a->D || ldy >= 1 << 26) return PSVAE_E_SHAPE;
+    if (ldy < a->D) return PSVAE_E_SHAPE;
     if (a->T > 0 && !y) return PSVAE_E_NULL;
     if (a->S == 0) return 0;
     const Plan p = scan_plan(a->T, a->S, a->D, a->G, a->N);
@@ -895,7 +903,7 @@ extern "C" int psvae_selective_scan_backward(const psvae_scan* a, const void* sa
     if (!g) return PSVAE_E_NULL;
     if (a->T > 0 && (!saved || !dy || !g->dx || !g->ddt || !g->dB || !g->dC || (a->z && !g->dz))) return PSVAE_E_NULL;
     if (!g->dA || !scratch) return PSVAE_E_NULL;
-    if (lddy < a->D || lddy >= 1 << 26) return PSVAE_E_SHAPE;
+    if (lddy < a->D) return PSVAE_E_SHAPE;
     const Plan p = scan_plan(a->T, a->S, a->D, a->G, a->N);
     Scan q = scan_args(a, p);
     const BwdScratch o = bwd_scratch(p, a->T, a->S, a->D, a->G);

@@ -167,12 +167,16 @@ class SSMBlock(nn.Module):
     def forward(self, x, seq_off=None, state=None, return_state=False):
         window, h0 = (None, None) if state is None else state
         u, z = ops.linear(self.norm(x), self.in_proj.weight).chunk(2, dim=-1)
-        v, window = ops.causal_conv(u, self.conv_weight, self.conv_bias, silu=True, seq_off=seq_off, state=window, return_state=True)
+        v = ops.causal_conv(u, self.conv_weight, self.conv_bias, silu=True, seq_off=seq_off, state=window, return_state=return_state)
+        if return_state:
+            v, window = v
         dt, B, C = self._split(v)
-        y, h = ops.selective_scan(v, dt, -torch.exp(self.A_log), B, C, D=self.D, z=z, dt_bias=self.dt_proj.bias, h0=h0, seq_off=seq_off,
-                                  return_state=True)
-        out = x + ops.linear(y, self.out_proj.weight)
-        return (out, (window, h)) if return_state else out
+        y = ops.selective_scan(v, dt, -torch.exp(self.A_log), B, C, D=self.D, z=z, dt_bias=self.dt_proj.bias, h0=h0, seq_off=seq_off,
+                               return_state=return_state)
+        if return_state:
+            y, h = y
+            return x + ops.linear(y, self.out_proj.weight), (window, h)
+        return x + ops.linear(y, self.out_proj.weight)
 
     @torch.no_grad()
     def step(self, x, state):

@@ -345,6 +345,60 @@ def test_offsets_that_lie_never_leave_the_rows():
         assert bool((pool == 3).all())
 
 
+def test_rows_outside_and_infinite_rates_stay_where_they_are():
+    """NaN and infinity in rows that no sequence holds reach nothing; a rate of -infinity forgets its state at every row
+    and nothing else, also where a sequence ends inside a tile."""
+    from ps_vae_amd import ops
+    off = torch.tensor([2, 13, 30], dtype=torch.int32, device=DEV)
+    dirty = _rand(1, 33, 24)
+    dirty[[0, 1, 30, 31, 32]] = torch.tensor([float('nan'), float('inf'), float('-inf'), float('nan'), float('inf')])[:, None]
+    clean = dirty.clone()
+    clean[[0, 1, 30, 31, 32]] = 0
+    A = -_rand(2, 24, 8).abs()
+    got = []
+    for x in (dirty, clean):
+        v, w, a = _gpu(x, grad=True), _gpu(_rand(3, 24, 4), grad=True), _gpu(A, grad=True)
+        u = ops.causal_conv(v, w, silu=True, seq_off=off)
+        y, last = ops.selective_scan(u, v, a, v[:, :8], v[:, 8:16], z=v, seq_off=off, return_state=True)
+        got.append([y, last, *torch.autograd.grad((y, last), (v, w, a), (_gpu(_rand(4, 33, 24)), torch.ones_like(last)))])
+    assert all(torch.equal(p, q) and bool(p.isfinite().all()) for p, q in zip(*got))
+    A[:, 3], x = float('-inf'), _gpu(clean[2:30])
+    y, last = ops.selective_scan(x, x, _gpu(A), x[:, :8], x[:, 8:16], h0=torch.ones(1, 24, 8, device=DEV), return_state=True)
+    step = torch.nn.functional.softplus(x[-1]) * x[-1]
+    assert bool(y.isfinite().all()) and torch.allclose(last[0, :, 3], step * x[-1, 3], rtol=1e-5, atol=1e-6)
+
+
+def test_more_elements_than_32_bits_count():
+    """2.2 G elements an operand: the last rows and sequences come out as they do by themselves, bit for bit."""
+    from ps_vae_amd import ops
+    S, L, D, few = 135_000, 16, 1024, 3
+    tail = [_gpu(_rand(i, few, L, D), torch.bfloat16) for i in range(2)]
+    x, dt = (torch.zeros(S, L, D, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    x[-few:], dt[-few:] = tail
+    w, A = _gpu(_rand(3, D, 4)), -_gpu(_rand(4, D, 1).abs())
+    ones = torch.ones(1, device=DEV, dtype=torch.bfloat16)
+
+    def run(x, dt):
+        x, dt = x.requires_grad_(), dt.requires_grad_()
+        bc = ones.expand(*x.shape[:2], 1)
+        n = ops.layer_norm(x)
+        u = ops.causal_conv(n, w, silu=True)
+        y, last = ops.selective_scan(u, dt, A, bc, bc, return_state=True)
+        dx, ddt = torch.autograd.grad(y, (x, dt), ones.expand_as(y))
+        return [q[-few:].clone() for q in (n, u, y, last, dx, ddt)]
+    alone = run(tail[0].clone(), tail[1].clone())
+    whole = run(x, dt)
+    assert x.numel() > 2 ** 31 and all(torch.equal(a, b) for a, b in zip(alone, whole))
+    state = torch.zeros(S, D, 16, device=DEV)                       # 2.2 G states, 8.8 GB
+    state[-few:] = 1
+    row = torch.ones(S, D, device=DEV, dtype=torch.bfloat16)
+    bc = torch.ones(S, 16, device=DEV, dtype=torch.bfloat16)
+    rates = A.expand(D, 16).contiguous()
+    y, _ = ops.selective_scan_step(row, row, rates, bc, bc, state)
+    ya, sa = ops.selective_scan_step(row[:few], row[:few], rates, bc[:few], bc[:few], torch.ones(few, D, 16, device=DEV))
+    assert torch.equal(y[-few:], ya) and torch.equal(state[-few:], sa)
+
+
 # ------------------------------------------------------------------ refusals
 
 def test_operators_refuse_what_they_do_not_take():
@@ -373,7 +427,13 @@ def test_operators_refuse_what_they_do_not_take():
     with pytest.raises(ValueError, match='overlaps'):
         ops.selective_scan_step(x, x, A, bc, bc, both[:6], state_out=both[1:])
     with pytest.raises(RuntimeError, match='no backward'):
-        ops.selective_scan_step(x.requires_grad_(), x, A, bc, bc, state)
+        ops.selective_scan_step(x.clone().requires_grad_(), x, A, bc, bc, state)
+    # gradients are not differentiable again: asking for a graph of them is fine, using it is refused
+    v = torch.ones(6, 8, device=DEV, requires_grad=True)
+    for y in (norm(v), conv(v, w + 1), scan(v, v, A - 1, bc + 1, bc + 1)):
+        g, = torch.autograd.grad((y * y).sum(), v, create_graph=True)
+        with pytest.raises(RuntimeError, match='once_differentiable'):
+            g.sum().backward()
 
 
 # ------------------------------------------------------------------ the operators together
@@ -481,6 +541,26 @@ def test_block_on_another_stream_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(eager, want[turn % 2]))
         for i in order:
             assert all(torch.equal(a, b) for a, b in zip(outs[i], want[(i + turn) % 2])), (turn, i)
+
+
+def test_block_captured_while_an_eager_graph_of_it_lives():
+    """A capture of forward and backward over aliases of the parameters (p.detach().requires_grad_()), while an eager graph
+    of the parameters themselves is alive: aliases have gradient nodes of their own, on the capturing stream."""
+    m = _block()
+    x = _gpu(_rand(1, 2, 30, 24))
+    params = dict(m.named_parameters())
+    alive = m(x)
+    want = torch.autograd.grad(alive, list(params.values()), torch.ones_like(alive), retain_graph=True)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        alias = {k: p.detach().requires_grad_() for k, p in params.items()}
+        y = torch.func.functional_call(m, alias, (x,))
+        got = torch.autograd.grad(y, list(alias.values()), torch.ones_like(y))
+    for _ in range(3):
+        g.replay()
+        again = torch.autograd.grad(alive, list(params.values()), torch.ones_like(alive), retain_graph=True)
+        torch.cuda.synchronize()
+        assert torch.equal(y, alive) and all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(got, want, again))
 
 
 def test_steps_in_a_graph():

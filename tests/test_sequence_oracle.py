@@ -103,7 +103,7 @@ def test_c_entry_points_refuse_bad_arguments():
         f = dict(x=p, dt=p, B=p, C=p, A=p, ldx=8, lddt=8, ldb=4, ldc=4, T=6, S=2, D=8, G=1, N=4, dtype=0, flags=2)
         return _lib.Scan(**{**f, **over})
     fwd = lambda **over: L.psvae_selective_scan_forward(scan(**over), p, 8, None, None, None, 0, None)  # noqa: E731
-    for bad in (dict(T=7), dict(N=0), dict(N=65, ldb=65, ldc=65), dict(G=3), dict(G=0), dict(D=0), dict(ldx=7), dict(ldx=1 << 26), dict(ldb=3), dict(dtype=9), dict(flags=1),
+    for bad in (dict(T=7), dict(N=0), dict(N=65, ldb=65, ldc=65), dict(G=3), dict(G=0), dict(D=0), dict(ldx=7), dict(ldb=3), dict(dtype=9), dict(flags=1),
                 dict(S=-1), dict(z=p, ldz=0)):
         assert fwd(**bad) == E_SHAPE, bad
     for bad in (dict(x=None), dict(A=None), dict(C=None)):
