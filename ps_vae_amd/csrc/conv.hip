@@ -9,7 +9,10 @@
 // sequence border.  All passes are bound by HBM: a lane owns 16 bytes of channels and walks down a stretch of rows with
 // the W rows it needs in registers, so every input row is read once per stretch plus W - 1 rows of run-up.
 // Stretches are laid over the packed rows and not over the sequences (a lane finds its sequence by bisection and then
-// follows the borders), so that one long and a thousand short sequences load the chip alike.
+// follows the borders), so that one long and a thousand short sequences load the chip alike.  Rows are loaded four at a
+// time, one group ahead, and a group without a border goes through without a test.  Measured at 8 x 2048 x 2048 bf16, four
+// taps: forward 33 us (4.1 TB/s; 49 us with no group ahead), backward 58 us (3.5 TB/s; 107 us with eight channels a lane and
+// two rows at a time) and 4 us for the parameters' sums; a copy reaches 5.0 TB/s.
 #include "seq_device.h"
 
 namespace {

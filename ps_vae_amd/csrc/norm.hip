@@ -6,7 +6,9 @@
 // Both passes are bound by HBM: forward moves x and y once, backward x, dy and dx once.  A row stays in the registers of
 // one wave (up to 256 vectors of 16 bytes) or of one workgroup (up to 2048 forward, 1024 backward), so the variance is
 // the second pass over registers of the two-pass formula (exact for rows whose mean is large against their spread) at no
-// further traffic.  Wider rows are read again for every pass (from L2).
+// further traffic.  Wider rows are read again for every pass (from L2).  Measured at 32768 x 2048 bf16: forward 57 us
+// (4.7 TB/s), backward 86 us (4.7 TB/s; 108 us before it loaded a row ahead) and 4 us for the parameters' sums; a copy
+// reaches 5.0 TB/s.  At 3277 x 300 fp32 the three kernels take 5, 7 and 4 us.
 #include "seq_device.h"
 
 namespace {

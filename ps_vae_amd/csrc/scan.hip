@@ -8,18 +8,24 @@
 //   dC[t, n] = sum_d h dyp      dB[t, n] = sum_d G delta x      dA[d, n] = sum_t G a h[t-1] delta
 //   dx = delta sum_n G B + D dyp      ddelta = x sum_n G B + sum_n G a h[t-1] A      dh0 = a[0] G[0]
 //
-// What bounds it: one exponential for every (row, channel, state) at a quarter of the vector rate, i.e. 16 cycles of a
-// SIMD for 64 of them, beside 4 cycles for each multiply-add: about 36 cycles forward and 90 backward for 64 cells, against
-// the 10 (22) bytes a channel and row that a 16-bit forward (backward) pass moves for 16 states.  No matrix instruction
-// helps: every channel and state has a decay of its own.
+// What bounds it: the vector units.  Every (row, channel, state) has a decay of its own, so no matrix product appears (and
+// forming delta A with the 4 x 4 x 1 matrix instruction cost more in waits than it saved: 159 against 146 us): 3 vector
+// operations and one exponential, which takes twice as long, for the state, one for y; backward 15 and one exponential.
+// With the sums, softplus and gates a forward pass issues 8.3 vector instructions a cell, a backward pass 25, and counters
+// show the vector units busy 93 % and 87 % of the time.  Measured at 16 states, bf16, 32 x 512 x 2048 (0.54 G cells): 146 us
+// forward (1.8 TB/s of its 4 operands) and 468 us backward; HBM alone would take 54 and 110 us.
 //
 // Layout: P lanes side by side share a channel and hold K states each (P K = the states rounded up: 4 x 1, 4 x 2, 4 x 4,
 // 8 x 4, 16 x 4), a workgroup of 256 lanes takes 256 / P channels of one group and one sequence and walks the time axis in
-// tiles of 16 rows: rows are read as vectors, brought to (delta, delta x, dyp) once, and passed to the lanes through LDS.
-// With the states of a channel spread over P lanes, the sum over the states costs log2 P steps inside the lanes' own row
-// (data-parallel moves, no LDS), and four times the workgroups of a lane-per-channel layout fill the chip at S x D = 8 k.
-// Few sequences: the time axis is cut into chunks (every sequence into as many), a first pass finds each chunk's end
-// state from zero, and the second, which makes the outputs, starts from the join of the chunks in front of it.
+// tiles of 16 rows: rows are read as vectors one tile ahead, brought to (delta, delta x, dyp) once, and passed to the lanes
+// through LDS.  With the states of a channel spread over P lanes, the sum over the states costs log2 P steps inside the
+// lanes' own row (data-parallel moves, no LDS), and four times the workgroups of a lane-per-channel layout fill the chip.
+// (8 x 2 and 16 x 1 for 16 states were slower wherever 4 x 4 was cut into pieces instead: 612 and 807 against 585 us for
+// the backward pass of 8 x 2048 x 2048.)  dB and dC are sums over channels: a fold over the halves of the wave and of its
+// halves (permlane swaps, which leave every lane half as many sums), then inside rows of 16 lanes, the waves through LDS and
+// the workgroups through memory, in a fixed order.
+// Few sequences: the time axis is cut into pieces ("chunks", every sequence into as many), a first pass finds each one's end
+// state from zero, and the second, which makes the outputs, starts from the join of the pieces in front of it.
 #include "seq_device.h"
 
 namespace {
@@ -332,7 +338,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Scan q) {
 
 // Backward.  CARRY: only what each chunk passes to the one in front of it, from a zero carry, and its sum of delta.
 template <class T, int P, int K, bool VEC, bool CARRY>
-__global__ __launch_bounds__(256, CARRY ? 4 : 2) void scan_bwd_kernel(Scan q) {
+__global__ __launch_bounds__(256, CARRY ? 3 : 2) void scan_bwd_kernel(Scan q) {
     using Sh = Shape<P, K>;
     constexpr int NP = Sh::NP, VE = Sh::VE, U = sizeof(T);
     // LDS, one block of constant parts: by channel what its lanes need of the rows (delta, delta x, dyp), what they make of
