@@ -8,7 +8,7 @@
 // the second pass over registers of the two-pass formula (exact for rows whose mean is large against their spread) at no
 // further traffic.  Wider rows are read again for every pass (from L2).  Measured at 32768 x 2048 bf16: forward 57 us
 // (4.7 TB/s), backward 86 us (4.7 TB/s; 108 us before it loaded a row ahead) and 4 us for the parameters' sums; a copy
-// reaches 5.0 TB/s.  At 3277 x 300 fp32 the three kernels take 5, 7 and 4 us.
+// reaches 5.0 TB/s.  At 3277 x 300 fp32 the three kernels take 5, 7 and 4 us, which the host's time to queue them hides.
 #include "seq_device.h"
 
 namespace {
@@ -118,13 +118,14 @@ __global__ __launch_bounds__(256) void norm_fwd_wide_kernel(const T* __restrict_
 }
 
 // dx, and this workgroup's part of dw and db.  A workgroup takes rows blockIdx.x * ROWS + (0 .. ROWS-1) and on in steps of
-// the grid, keeps its columns' sums in registers, joins its waves through LDS and writes partial[blockIdx.x][2][H]: the
-// parameter gradients cost one pass of 2 H floats per workgroup and no atomics (the order of every sum is fixed).
+// the grid, keeps its columns' sums in registers, joins its waves through LDS and writes them 2 H floats further for every
+// workgroup: the parameter gradients cost one pass of 2 H floats per workgroup and no atomics (the order of every sum is
+// fixed).  A single workgroup writes the gradients themselves.
 template <class T, int V, int WPR, int IT>
 __global__ __launch_bounds__(256) void norm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx,
                                                        const float* __restrict__ w, const float* __restrict__ mean,
                                                        const float* __restrict__ rstd, T* __restrict__ dx, int64_t lddx,
-                                                       float* __restrict__ partial, int rows, int H) {
+                                                       float* __restrict__ dw_out, float* __restrict__ db_out, int rows, int H) {
     extern __shared__ float join[];                    // 2 H floats (WPR 1) or 8 (WPR 4)
     constexpr int ROWS = WPR == 1 ? 4 : 1;
     const int lane = WPR == 1 ? threadIdx.x & 63 : threadIdx.x, wave = threadIdx.x >> 6;
@@ -199,8 +200,8 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(const T* __restrict__ dy,
             store_vec<V>(dx + row * lddx + c, o);
         }
     }
-    if (!partial) return;
-    float* out = partial + (int64_t)blockIdx.x * 2 * H;
+    if (!dw_out && !db_out) return;
+    const int64_t part = (int64_t)blockIdx.x * 2 * H;
     if constexpr (WPR == 1) {
         for (int turn = 0; turn < 4; ++turn) {
             if (wave == turn) {
@@ -217,15 +218,20 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(const T* __restrict__ dy,
             }
             __syncthreads();
         }
-        for (int c = threadIdx.x; c < 2 * H; c += 256) out[c] = join[c];
+        for (int c = threadIdx.x; c < H; c += 256) {
+            if (dw_out) dw_out[part + c] = join[c];
+            if (db_out) db_out[part + c] = join[H + c];
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int c = (i * 256 + lane) * V;
             if (c >= H) continue;
-            store_vec<V>(out + c, dw[i]);
 #pragma unroll
-            for (int k = 0; k < V; ++k) out[H + c + k] = db[i][k];
+            for (int k = 0; k < V; ++k) {
+                if (dw_out) dw_out[part + c + k] = dw[i][k];
+                if (db_out) db_out[part + c + k] = db[i][k];
+            }
         }
     }
 }
@@ -316,8 +322,9 @@ __global__ __launch_bounds__(256) void column_sums_kernel(const float* __restric
 constexpr int NORM_PARTS = 512;   // workgroups of the backward pass: two for every CU
 
 int norm_parts(int64_t rows) {
-    // eight rows to a workgroup before another one is added: the partial sums are 2 H floats each
-    const int64_t want = (rows + 7) / 8;
+    // one workgroup for a few rows (no second launch to join the parts); else eight rows to a workgroup before another one
+    // is added: the partial sums are 2 H floats each
+    const int64_t want = rows <= 16 ? 1 : (rows + 7) / 8;
     return (int)(want < 1 ? 1 : (want > NORM_PARTS ? NORM_PARTS : want));
 }
 
@@ -345,9 +352,11 @@ template <class T, int V> int norm_bwd(hipStream_t s, const T* dy, int64_t lddy,
     const int nvec = H / V;
     const int parts = norm_parts(rows);
     float* part = dw || db ? partial : nullptr;
+    const bool one = parts == 1;
+    float *dw_to = one ? dw : part, *db_to = one ? db : (part ? part + H : nullptr);
 #define PSVAE_NORM_BWD(WPR, IT)                                                                                            \
     hipLaunchKernelGGL((norm_bwd_kernel<T, V, WPR, IT>), dim3(parts), dim3(256), (WPR == 1 ? 2 * H : 8) * sizeof(float), s, dy, \
-                       lddy, x, ldx, w, mean, rstd, dx, lddx, part, rows, H)
+                       lddy, x, ldx, w, mean, rstd, dx, lddx, dw_to, db_to, rows, H)
     if (nvec <= 64) PSVAE_NORM_BWD(1, 1);
     else if (nvec <= 128) PSVAE_NORM_BWD(1, 2);
     else if (nvec <= 256) PSVAE_NORM_BWD(1, 4);
@@ -360,7 +369,7 @@ template <class T, int V> int norm_bwd(hipStream_t s, const T* dy, int64_t lddy,
     }
 #undef PSVAE_NORM_BWD
     PSVAE_LAUNCH_CHECK();
-    return part ? column_sums(s, part, parts, H, 1, dw, db) : 0;
+    return part && !(one && nvec <= 1024) ? column_sums(s, part, parts, H, 1, dw, db) : 0;
 }
 
 }  // namespace
