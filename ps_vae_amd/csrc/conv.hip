@@ -17,7 +17,8 @@
 
 namespace {
 
-// The sequence that row t belongs to: the last one that begins at or before t and is not empty behind t.
+// The sequence that row t belongs to: the last one that begins at or before t and is not empty behind t.  Behind the last
+// one it is S, which begins so far off that no row counts as one in front of it (it has no state).
 struct Walk { int s, begin, end; };
 __device__ __forceinline__ Walk walk_to(const int32_t* off, int S, int T, int t) {
     if (!off) {
@@ -29,7 +30,7 @@ __device__ __forceinline__ Walk walk_to(const int32_t* off, int S, int T, int t)
         const int mid = (lo + hi) >> 1;
         if (off[mid + 1] > t) hi = mid; else lo = mid + 1;
     }
-    if (lo == S) return {S, T, T};
+    if (lo == S) return {S, INT32_MAX - 16, INT32_MAX - 16};
     const SeqBounds b = seq_bounds(off, lo, S, T);
     return {lo, b.begin, b.end};
 }

@@ -183,6 +183,26 @@ def test_causal_conv_prompt_then_steps(kind, D, W):
     assert torch.equal(torch.cat(got, 1), whole) and torch.equal(state, end)
 
 
+@pytest.mark.parametrize('kind,D,W', [('f32', 8, 4), ('bf16', 64, 3), ('f16', 9, 8)])
+def test_causal_conv_rows_behind_the_last_sequence_have_no_state(kind, D, W):
+    """A stretch of rows that begins behind the last sequence, less than W - 1 rows from the end, has no state to read: what
+    lies behind the states in memory reaches nothing."""
+    from ps_vae_amd import ops
+    t = TYPES[kind]
+    states = torch.full((4, W - 1, D), float('nan'), device=DEV, dtype=t)
+    states[:2] = _gpu(_rand(1, 2, W - 1, D), t)
+    x, dy, w, b = _gpu(_rand(2, 66, D), t), _gpu(_rand(3, 66, D), t), _gpu(_rand(4, D, W), grad=True), _gpu(_rand(5, D), grad=True)
+    off = torch.tensor([0, 3, 64], dtype=torch.int32, device=DEV)
+    got = []
+    for rows in (64, 65, 66):
+        v = x[:rows].detach().requires_grad_()
+        y = ops.causal_conv(v, w, b, silu=True, seq_off=off, state=states[:2])
+        dx, dw, db = torch.autograd.grad(y, (v, w, b), dy[:rows])
+        assert bool((y[64:] == 0).all()) and bool((dx[64:] == 0).all())
+        got.append((y[:64], dx[:64], dw, db))
+    assert all(torch.equal(p, q) and bool(p.isfinite().all()) for other in got[1:] for p, q in zip(got[0], other))
+
+
 # ------------------------------------------------------------------ scan
 
 SCAN_CASES = [   # (lengths, first row, rows behind, width, states, groups, type, flags: z D bias h0 softplus)
