@@ -123,13 +123,13 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(const T* __restrict__ x, 
 template <class T>
 __global__ __launch_bounds__(256) void conv_state_kernel(const T* __restrict__ x, int64_t ldx, const int32_t* __restrict__ off,
                                                          const T* __restrict__ state, T* __restrict__ out, int S, int T_, int D, int back) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (int64_t)S * back * D) return;
-    const int d = (int)(i % D), k = (int)(i / D % back), s = (int)(i / ((int64_t)D * back));
-    const SeqBounds q = seq_bounds(off, s, S, T_);
-    const int t = q.end - back + k;
-    out[i] = t >= q.begin ? x[(int64_t)t * ldx + d]
-                          : (state ? state[((int64_t)s * back + back - (q.begin - t)) * D + d] : (T)0.f);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)S * back * D; i += (int64_t)gridDim.x * 256) {
+        const int d = (int)(i % D), k = (int)(i / D % back), s = (int)(i / ((int64_t)D * back));
+        const SeqBounds q = seq_bounds(off, s, S, T_);
+        const int t = q.end - back + k;
+        out[i] = t >= q.begin ? x[(int64_t)t * ldx + d]
+                              : (state ? state[((int64_t)s * back + back - (q.begin - t)) * D + d] : (T)0.f);
+    }
 }
 
 // dx, and this workgroup's part of dw and db: partial[blockIdx.x][W + 1][D].  The pre-activation is computed again from
@@ -277,24 +277,24 @@ __global__ __launch_bounds__(256) void conv_step_kernel(const T* __restrict__ x,
                                                         const float* __restrict__ w, const float* __restrict__ b, T* __restrict__ y,
                                                         int64_t ldy, int S, int D, int flags) {
     const int per = D / V;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (int64_t)S * per) return;
-    const int64_t s = i / per;
-    const int c = (int)(i - s * per) * V;
-    float win[W][V], o[V];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)S * per; i += (int64_t)gridDim.x * 256) {
+        const int64_t s = i / per;
+        const int c = (int)(i - s * per) * V;
+        float win[W][V], o[V];
 #pragma unroll
-    for (int k = 0; k + 1 < W; ++k) load_vec<V>(state + (s * (W - 1) + k) * D + c, win[k]);
-    load_vec<V>(x + s * ldx + c, win[W - 1]);
+        for (int k = 0; k + 1 < W; ++k) load_vec<V>(state + (s * (W - 1) + k) * D + c, win[k]);
+        load_vec<V>(x + s * ldx + c, win[W - 1]);
 #pragma unroll
-    for (int i2 = 0; i2 < V; ++i2) {
-        float pre = b ? b[c + i2] : 0.f;
+        for (int i2 = 0; i2 < V; ++i2) {
+            float pre = b ? b[c + i2] : 0.f;
 #pragma unroll
-        for (int k = 0; k < W; ++k) pre = fmaf(w[(int64_t)(c + i2) * W + k], win[k][i2], pre);
-        o[i2] = flags & PSVAE_SEQ_SILU ? pre * sigmoidf(pre) : pre;
+            for (int k = 0; k < W; ++k) pre = fmaf(w[(int64_t)(c + i2) * W + k], win[k][i2], pre);
+            o[i2] = flags & PSVAE_SEQ_SILU ? pre * sigmoidf(pre) : pre;
+        }
+        store_vec<V>(y + s * ldy + c, o);
+#pragma unroll
+        for (int k = 0; k + 1 < W; ++k) store_vec<V>(state_out + (s * (W - 1) + k) * D + c, win[k + 1]);
     }
-    store_vec<V>(y + s * ldy + c, o);
-#pragma unroll
-    for (int k = 0; k + 1 < W; ++k) store_vec<V>(state_out + (s * (W - 1) + k) * D + c, win[k + 1]);
 }
 
 // Lanes side by side in a row: the smallest power of two that covers the channels, at most a wave (whose access is then
@@ -315,6 +315,8 @@ int conv_rows(int64_t T, int nvec, int lanes) {
 // filters and sums would otherwise leave registers for a single wave of a SIMD.
 int conv_vec(int dtype, int W, bool backward) { return dtype == PSVAE_F32 || backward || W > 4 ? 4 : 8; }
 
+unsigned blocks_of(int64_t n) { return (unsigned)((n + 255) / 256 < MOST_BLOCKS ? (n + 255) / 256 : MOST_BLOCKS); }
+
 struct ConvPlan { ConvShape q; int V, gx, gy; };
 ConvPlan conv_plan(int64_t T, int D, int S, int V, int flags) {
     const int nvec = (D + V - 1) / V, lanes = conv_lanes(nvec), R = conv_rows(T, nvec, lanes);
@@ -333,7 +335,7 @@ template <class T, int V, int W> struct ConvRun {
     static int step(hipStream_t s, const void* x, int64_t ldx, const void* state, void* state_out, const float* w, const float* b, void* y,
                     int64_t ldy, int S, int D, int flags) {
         const int64_t n = (int64_t)S * (D / V);
-        hipLaunchKernelGGL((conv_step_kernel<T, V, W>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, (const T*)x, ldx, (const T*)state,
+        hipLaunchKernelGGL((conv_step_kernel<T, V, W>), dim3(blocks_of(n)), dim3(256), 0, s, (const T*)x, ldx, (const T*)state,
                            (T*)state_out, w, b, (T*)y, ldy, S, D, flags);
         PSVAE_LAUNCH_CHECK();
         return 0;
@@ -389,7 +391,7 @@ extern "C" int psvae_causal_conv_forward(const void* x, int64_t ldx, const float
     if (state_out && S > 0 && W > 1) {
         const int64_t n = (int64_t)S * (W - 1) * D;
         PSVAE_BY_TYPE(dtype, E, {
-            hipLaunchKernelGGL((conv_state_kernel<E>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, (const E*)x, ldx, seq_off,
+            hipLaunchKernelGGL((conv_state_kernel<E>), dim3(blocks_of(n)), dim3(256), 0, s, (const E*)x, ldx, seq_off,
                                (const E*)state, (E*)state_out, S, (int)T, D, W - 1);
         });
         PSVAE_LAUNCH_CHECK();

@@ -363,7 +363,9 @@ template <class T, int V> int norm_bwd(hipStream_t s, const T* dy, int64_t lddy,
     else if (nvec <= 512) PSVAE_NORM_BWD(4, 2);
     else if (nvec <= 1024) PSVAE_NORM_BWD(4, 4);
     else {
-        if (dx) hipLaunchKernelGGL((norm_bwd_wide_kernel<T, V>), dim3(rows), dim3(256), 0, s, dy, lddy, x, ldx, w, mean, rstd, dx, lddx, H);
+        for (int64_t r = 0; dx && r < rows; r += MOST_BLOCKS)
+            hipLaunchKernelGGL((norm_bwd_wide_kernel<T, V>), dim3((unsigned)(rows - r < MOST_BLOCKS ? rows - r : MOST_BLOCKS)), dim3(256), 0, s,
+                               dy + r * lddy, lddy, x + r * ldx, ldx, w, mean + r, rstd + r, dx + r * lddx, lddx, H);
         if (part) hipLaunchKernelGGL((norm_param_grad_kernel<T, V>), dim3(parts, (nvec + 255) / 256), dim3(256), 0, s, dy, lddy, x, ldx,
                                      mean, rstd, part, rows, H);
     }
@@ -399,8 +401,15 @@ extern "C" int psvae_layer_norm_forward(const void* x, int64_t ldx, const float*
     ProfScope prof(s, KC_NORM, 2.0 * rows * width * dtype_bytes(dtype));
     PSVAE_BY_TYPE(dtype, T, {
         constexpr int V = 16 / sizeof(T);
-        return vec ? norm_fwd<T, V>(s, (const T*)x, ldx, weight, bias, (T*)y, ldy, mean, rstd, (int)rows, width, eps)
-                   : norm_fwd<T, 1>(s, (const T*)x, ldx, weight, bias, (T*)y, ldy, mean, rstd, (int)rows, width, eps);
+        for (int64_t r = 0; r < rows; r += MOST_BLOCKS) {
+            const int n = (int)(rows - r < MOST_BLOCKS ? rows - r : MOST_BLOCKS);
+            const T* from = (const T*)x + r * ldx;
+            T* to = (T*)y + r * ldy;
+            float *const m = mean ? mean + r : nullptr, *const sd = rstd ? rstd + r : nullptr;
+            PSVAE_TRY((vec ? norm_fwd<T, V>(s, from, ldx, weight, bias, to, ldy, m, sd, n, width, eps)
+                           : norm_fwd<T, 1>(s, from, ldx, weight, bias, to, ldy, m, sd, n, width, eps)));
+        }
+        return 0;
     });
 }
 

@@ -838,9 +838,21 @@ template <class T, int P, int K> int fwd_run(hipStream_t s, const Scan& q, const
 template <class T, int P, int K> int bwd_run(hipStream_t s, const Scan& q, const Plan& p) {
     return q.vec ? bwd_run_as<T, P, K, true>(s, q, p) : bwd_run_as<T, P, K, false>(s, q, p);
 }
-template <class T, int P, int K> int step_run(hipStream_t s, const Scan& q, const Plan&) {
+template <class T, int P, int K> int step_run(hipStream_t s, const Scan& whole, const Plan& p) {
+    Scan q = whole;
     const int vec = q.N == P * K && rows_vec(q.A, 0, K, PSVAE_F32) && rows_vec(q.h0, 0, K, PSVAE_F32) && rows_vec(q.hT, 0, K, PSVAE_F32);
-    const int64_t wide = (q.Dn * P + 255) / 256;
+    const int64_t wide = (q.Dn * P + 255) / 256, most = MOST_BLOCKS / wide;
+    if (q.S > most) {                                   // more than one launch holds: the others in further ones
+        q.S = (int)most;
+        PSVAE_TRY((step_run<T, P, K>(s, q, p)));
+        q.S = (int)(whole.S - most);
+        const auto on = [&](const void* v, int64_t ld) -> const void* { return v ? (const T*)v + most * ld : nullptr; };
+        q.x = on(q.x, q.ldx); q.dt = on(q.dt, q.lddt); q.z = on(q.z, q.ldz); q.B = on(q.B, q.ldb); q.C = on(q.C, q.ldc);
+        q.y = (T*)q.y + most * q.ldy;
+        q.h0 += most * q.Dn * q.N;
+        q.hT += most * q.Dn * q.N;
+        return step_run<T, P, K>(s, q, p);
+    }
     // four sequences a lane where that leaves two workgroups for every CU
     if (wide * ((q.S + 3) / 4) >= 512)
         hipLaunchKernelGGL((scan_step_kernel<T, P, K, 4>), dim3((unsigned)(wide * ((q.S + 3) / 4))), dim3(256), 0, s, q, vec);

@@ -9,6 +9,8 @@ typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 
 static inline size_t dtype_bytes(int dtype) { return dtype == PSVAE_F32 ? 4 : 2; }
+// A launch has fewer than 2^32 threads: work beyond this many workgroups of 256 goes into further launches or a loop.
+constexpr int64_t MOST_BLOCKS = 1 << 23;
 static inline bool dtype_known(int dtype) { return dtype == PSVAE_F32 || dtype == PSVAE_BF16 || dtype == PSVAE_F16; }
 
 template <class T, int V> struct VecOf { typedef T type __attribute__((ext_vector_type(V))); };

@@ -419,6 +419,39 @@ def test_more_elements_than_32_bits_count():
     assert torch.equal(y[-few:], ya) and torch.equal(state[-few:], sa)
 
 
+def test_more_work_than_one_launch_takes():
+    """Rows and sequences beyond 2^23 workgroups go into further launches or turns: the last ones come out as they do by
+    themselves, bit for bit."""
+    from ps_vae_amd import ops
+    few, bf16 = 5, torch.bfloat16
+
+    def zeros(rows, *shape):
+        v = torch.zeros(rows, *shape, device=DEV, dtype=bf16)
+        v[-few:] = _gpu(_rand(1, few, *shape), bf16)
+        return v
+
+    def alike(f, x):
+        for whole, alone in zip(f(x), f(x[-few:].clone())):
+            assert bool(alone.isfinite().all()) and torch.equal(whole[-few:], alone)
+
+    def norm(x):
+        x = x.detach().requires_grad_()
+        y = ops.layer_norm(x)
+        return y.detach(), torch.autograd.grad(y, x, x.detach())[0]
+    for rows, width in ((1 << 25, 8), (1 << 23, 257), (1 << 23, 1025)):   # a wave, a workgroup a row; backward in two readings
+        alike(norm, zeros(rows + few + 3, width))
+    D = 1025
+    w = _gpu(_rand(2, D, 8))
+    alike(lambda x: ops.causal_conv_step(x, torch.empty(len(x), 0, D, device=DEV, dtype=bf16), w[:, :1].contiguous())[:1], zeros((1 << 21) + few, D))
+    alike(lambda x: ops.causal_conv(x, w[:160], return_state=True), zeros((1 << 21) + few, 1, 160))
+    A = -_gpu(_rand(3, 1024, 1).abs())
+
+    def step(x):
+        state = torch.ones(len(x), 1024, 1, device=DEV)
+        return ops.selective_scan_step(x, x, A, x[:, :1], x[:, 1:2], state, z=x)
+    alike(step, zeros((1 << 19) + few, 1024))
+
+
 # ------------------------------------------------------------------ refusals
 
 def test_operators_refuse_what_they_do_not_take():
