@@ -127,7 +127,8 @@ class SSMBlock(nn.Module):
         out = x + out_proj(selective_scan(v, dt_proj(r), -exp(A_log), B, C, D, gate z))
 
     `forward` takes [S, L, dim], or packed rows [T, dim] with `seq_off` (int32 [S+1]); `step` one row for each of S
-    sequences, with a state from `init_state` or from `forward(.., return_state=True)`.  fp32, as the Linear kernels."""
+    sequences, with a state from `init_state` or from `forward(.., return_state=True)`.  fp32 and at least one row, as the
+    Linear kernels."""
 
     def __init__(self, dim, dim_inner=None, num_states=16, num_taps=4, dt_rank=None, num_groups=1):
         super().__init__()

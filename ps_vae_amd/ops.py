@@ -187,6 +187,12 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _written(t):
+    """Tells autograd that the library wrote into `t`, so that a backward pass that kept it says so instead of using it."""
+    if not t.is_inference():                               # those have no version to count
+        torch.autograd.graph.increment_version(t)
+
+
 def _rows(t, width):
     """`t` as rows of `width` contiguous elements and the distance of two rows; a copy only where no view does it."""
     if t.is_contiguous():
@@ -392,6 +398,7 @@ def causal_conv_step(x, state, weight, bias=None, *, silu=False, state_out=None)
     y = torch.empty(S, D, dtype=x.dtype, device=x.device)
     _run('psvae_causal_conv_step', x.device, _lib.lib().psvae_causal_conv_step, x2.data_ptr(), ldx, state.data_ptr(), out.data_ptr(), weight.data_ptr(),
          _ptr(bias), y.data_ptr(), D, S, D, weight.shape[1], _DTYPES[x.dtype], _lib.SEQ_SILU if silu else 0)
+    _written(out)
     return y, out
 
 
@@ -535,4 +542,5 @@ def selective_scan_step(x, dt, A, B, C, state, *, D=None, z=None, dt_bias=None, 
     a = _scan_call(x2, dt2, A, B2, C2, D, z2, dt_bias, state, None, ld, S, S, G, _lib.SEQ_SOFTPLUS if softplus else 0)
     y = torch.empty(S, width, dtype=x.dtype, device=x.device)
     _run('psvae_selective_scan_step', x.device, _lib.lib().psvae_selective_scan_step, a, y.data_ptr(), width, out.data_ptr())
+    _written(out)
     return y, out

@@ -635,3 +635,27 @@ def test_steps_in_a_graph():
         g.replay()
         assert torch.equal(y, want[i])
     assert all(torch.equal(a, b) for a, b in zip(state, eager))
+
+
+def test_steps_in_place_are_seen_by_a_backward_pass_that_kept_the_state():
+    """A state that a convolution's backward pass reads and a token step has moved on since is refused, not used; in
+    inference mode, where nothing is kept, steps go on."""
+    from ps_vae_amd import ops
+    x, w = _gpu(_rand(1, 2, 5, 8), grad=True), _gpu(_rand(2, 8, 4))
+    A, bc = -torch.ones(8, 4, device=DEV), torch.ones(2, 4, device=DEV)
+    for into in (False, True):
+        state = torch.ones(2, 3, 8, device=DEV)
+        y = ops.causal_conv(x, w, state=state)
+        ops.causal_conv_step(x[:, 0].detach(), state.clone() if into else state, w, state_out=state if into else None)
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            y.sum().backward()
+    h = torch.ones(2, 8, 4, device=DEV)
+    kept = (h * h.clone().requires_grad_()).sum()
+    ops.selective_scan_step(x[:, 0].detach(), x[:, 1].detach(), A, bc, bc, h)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        kept.backward()
+    with torch.inference_mode():
+        state = torch.ones(2, 3, 8, device=DEV)
+        before = state.clone()
+        ops.causal_conv_step(x[:, 0].detach(), state, w)
+        assert not torch.equal(state, before)
