@@ -659,3 +659,29 @@ def test_steps_in_place_are_seen_by_a_backward_pass_that_kept_the_state():
         before = state.clone()
         ops.causal_conv_step(x[:, 0].detach(), state, w)
         assert not torch.equal(state, before)
+
+
+@pytest.mark.parametrize('shape', [(0, 5, 8), (2, 0, 8), (0, 8)])
+def test_no_rows_give_no_rows_and_zero_gradients(shape):
+    """No sequences, or only empty ones; the block's Linear kernels refuse what has no rows, before a state is touched."""
+    from ps_vae_amd import ops
+    off = torch.zeros(1, dtype=torch.int32, device=DEV) if len(shape) == 2 else None
+    S = shape[0]
+    x, w, A = torch.zeros(shape, device=DEV, requires_grad=True), torch.ones(8, 4, device=DEV, requires_grad=True), -torch.ones(8, 2, device=DEV)
+    A.requires_grad_()
+    h0, bc = torch.ones(S, 8, 2, device=DEV, requires_grad=True), torch.zeros(*shape[:-1], 2, device=DEV)
+    gain = torch.ones(8, device=DEV, requires_grad=True)
+    u, end = ops.causal_conv(ops.layer_norm(x, gain, gain), w, seq_off=off, state=torch.ones(S, 3, 8, device=DEV), return_state=True)
+    y, last = ops.selective_scan(u, u, A, bc, bc, D=gain, h0=h0, seq_off=off, return_state=True)
+    assert y.shape == shape and bool((end == 1).all()) and end.shape == (S, 3, 8) and torch.equal(last, h0)
+    grads = torch.autograd.grad(y.sum() + last.sum(), (x, w, A, gain, h0))
+    assert [g.shape for g in grads] == [v.shape for v in (x, w, A, gain, h0)]
+    assert all(bool((g == 0).all()) for g in grads[:4]) and bool((grads[4] == 1).all())
+    rows = torch.zeros(0, 8, device=DEV)
+    with torch.no_grad():
+        ops.causal_conv_step(rows, torch.ones(0, 3, 8, device=DEV), w)
+        ops.selective_scan_step(rows, rows, A, rows[:, :2], rows[:, :2], torch.ones(0, 8, 2, device=DEV))
+        m, state = _block(8), torch.ones(shape[0], 3, 16, device=DEV)
+        with pytest.raises(RuntimeError):
+            m(x, seq_off=off, state=(state, torch.ones(shape[0], 16, 16, device=DEV)))
+        assert bool((state == 1).all())
