@@ -1,6 +1,7 @@
 """Single-operator autograd functions over the C ABI (the module-level API uses
 these; the whole-step path in `model.py` bypasses them)."""
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -250,6 +251,16 @@ def _sequences(what, x, seq_off):
     return rows, seq_off.numel() - 1
 
 
+def _no_tangent(what, *tensors):
+    """Refuses operands of forward-mode differentiation: the kernels read the values alone, and a result without a tangent
+    would stand for a derivative of zero."""
+    # no level is open almost always; unpacking nine operands to find that out would cost as much as a launch
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f'{what} has no forward-mode derivative: its operands must not carry tangents')
+
+
 def _wants_grad(*tensors):
     if torch.is_grad_enabled():
         for t in tensors:
@@ -308,6 +319,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     _first('layer_norm', x, 1, 64)
     shape = x.shape[-1:]
     weight, bias = _par('layer_norm', 'weight', weight, x, shape), _par('layer_norm', 'bias', bias, x, shape)
+    _no_tangent('layer_norm', x, weight, bias)
     if _wants_grad(x, weight, bias):
         return LayerNormFn.apply(x, weight, bias, float(eps))
     return _norm_forward(x, weight, bias, float(eps), False)[0]
@@ -375,6 +387,7 @@ def causal_conv(x, weight, bias=None, *, silu=False, seq_off=None, state=None, r
         if state.requires_grad:
             raise ValueError(f'{what}: no gradient is computed for the state; pass state.detach()')
         state = state.contiguous()
+    _no_tangent(what, x, weight, bias, state)
     flags = (_lib.SEQ_SILU if silu else 0) | (_lib.SEQ_ZERO_OUTSIDE if seq_off is not None else 0)
     if _wants_grad(x, weight, bias):
         y, out = CausalConvFn.apply(x, weight, bias, state, seq_off, flags, rows, S, bool(return_state))
@@ -390,6 +403,7 @@ def causal_conv_step(x, state, weight, bias=None, *, silu=False, state_out=None)
     _first(what, x, 2, 2)
     S, D = x.shape
     weight, bias = _conv_params(what, x, weight, bias)
+    _no_tangent(what, x, state, weight, bias, state_out)
     if _wants_grad(x, state, weight, bias):
         raise RuntimeError(f'{what} has no backward pass: call it under torch.no_grad() or on detached tensors')
     _act(what, 'state', state, x, (S, weight.shape[1] - 1, D))
@@ -518,6 +532,7 @@ def selective_scan(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, softplus=Tru
     _first(what, x, 2, 3)
     rows, S = _sequences(what, x, seq_off)
     A, D, dt_bias, h0, G = _scan_operands(what, x, dt, A, B, C, D, z, dt_bias, h0, S)
+    _no_tangent(what, x, dt, A, B, C, D, z, dt_bias, h0)
     flags = (_lib.SEQ_SOFTPLUS if softplus else 0) | (_lib.SEQ_ZERO_OUTSIDE if seq_off is not None else 0)
     if _wants_grad(x, dt, A, B, C, D, z, dt_bias, h0):
         y, last = SelectiveScanFn.apply(x, dt, A, B, C, D, z, dt_bias, h0, seq_off, flags, rows, S, G, bool(return_state))
@@ -534,6 +549,7 @@ def selective_scan_step(x, dt, A, B, C, state, *, D=None, z=None, dt_bias=None, 
     S, width = x.shape
     if state.dtype != torch.float32:
         raise ValueError(f'{what}: state is {state.dtype}, expected torch.float32')
+    _no_tangent(what, x, dt, A, B, C, state, D, z, dt_bias, state_out)
     if _wants_grad(x, dt, A, B, C, state, D, z, dt_bias):
         raise RuntimeError(f'{what} has no backward pass: call it under torch.no_grad() or on detached tensors')
     out = _state_out(what, state, state_out)
