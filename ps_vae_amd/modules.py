@@ -128,7 +128,11 @@ class SSMBlock(nn.Module):
 
     `forward` takes [S, L, dim], or packed rows [T, dim] with `seq_off` (int32 [S+1]); `step` one row for each of S
     sequences, with a state from `init_state` or from `forward(.., return_state=True)`.  fp32 and at least one row, as the
-    Linear kernels."""
+    Linear kernels.
+
+    Training in segments cuts the gradient at their borders: no gradient passes through the convolution's part of a state
+    (its last rows), so `forward` takes a returned state only detached, both parts of it unless the other one's share by
+    itself is meant."""
 
     def __init__(self, dim, dim_inner=None, num_states=16, num_taps=4, dt_rank=None, num_groups=1):
         super().__init__()
@@ -167,6 +171,8 @@ class SSMBlock(nn.Module):
 
     def forward(self, x, seq_off=None, state=None, return_state=False):
         window, h0 = (None, None) if state is None else state
+        if window is not None and window.requires_grad and torch.is_grad_enabled():
+            raise ValueError('SSMBlock: no gradient passes through the convolution\'s part of a state; pass both parts detached')
         u, z = ops.linear(self.norm(x), self.in_proj.weight).chunk(2, dim=-1)
         v = ops.causal_conv(u, self.conv_weight, self.conv_bias, silu=True, seq_off=seq_off, state=window, return_state=return_state)
         if return_state:

@@ -336,20 +336,25 @@ def _conv_forward(x, w, b, state, seq_off, flags, rows, S, want_state):
 
 
 class CausalConvFn(torch.autograd.Function):
-    """y[t] = act(b + sum_k w[:, k] x[t - W + 1 + k]) inside every sequence; returns (y, final state or None)."""
+    """y[t] = act(b + sum_k w[:, k] x[t - W + 1 + k]) inside every sequence; returns (y, final state or None).  The state has
+    no gradient: backward refuses one."""
 
     @staticmethod
     def forward(ctx, x, w, b, state, seq_off, flags, rows, S, want_state):
         y, out, x2, ldx = _conv_forward(x, w, b, state, seq_off, flags, rows, S, want_state)
         ctx.save_for_backward(x2, w, b, state, seq_off)
         ctx.call = ldx, flags, rows, S, x.shape
-        if out is not None:
+        ctx.set_materialize_grads(False)
+        # the state holds rows of x: it requires a gradient as they do, so that one that is passed on is noticed
+        if out is not None and not (out.shape[1] and ctx.needs_input_grad[0]):
             ctx.mark_non_differentiable(out)
         return y, out
 
     @staticmethod
     @_once
-    def backward(ctx, dy, _):
+    def backward(ctx, dy, dout):
+        if dout is not None:
+            raise RuntimeError('causal_conv: no gradient is computed for the state; detach it')
         L = _lib.lib()
         x2, w, b, state, seq_off = ctx.saved_tensors
         ldx, flags, rows, S, shape = ctx.call
@@ -377,14 +382,15 @@ def _conv_params(what, x, weight, bias):
 def causal_conv(x, weight, bias=None, *, silu=False, seq_off=None, state=None, return_state=False):
     """Short causal convolution along every sequence, one filter a channel: weight [D, W] with 1 to 8 taps (the last one
     on the row itself), bias [D].  `state` [S, W-1, D] in x's type holds the inputs in front of every sequence (oldest
-    first; zeros without it) and carries no gradient; with `return_state` the call gives (y, state behind the end)."""
+    first; zeros without it); with `return_state` the call gives (y, state behind the end).  No gradient is computed for a
+    state: where one would be needed the call refuses, so the returned state is passed on as state.detach()."""
     what = 'causal_conv'
     _first(what, x, 2, 3)
     rows, S = _sequences(what, x, seq_off)
     weight, bias = _conv_params(what, x, weight, bias)
     if state is not None:
         _act(what, 'state', state, x, (S, weight.shape[1] - 1, x.shape[-1]))
-        if state.requires_grad:
+        if _wants_grad(state):
             raise ValueError(f'{what}: no gradient is computed for the state; pass state.detach()')
         state = state.contiguous()
     _no_tangent(what, x, weight, bias, state)

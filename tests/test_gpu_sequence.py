@@ -685,3 +685,23 @@ def test_no_rows_give_no_rows_and_zero_gradients(shape):
         with pytest.raises(RuntimeError):
             m(x, seq_off=off, state=(state, torch.ones(shape[0], 16, 16, device=DEV)))
         assert bool((state == 1).all())
+
+
+def test_block_trained_in_segments_cuts_the_gradient_at_their_border():
+    """Two segments with a detached state between them: the loss of the whole sequence, each parameter's gradient the sum of
+    the two segments' own.  A state that is not detached is refused, in the next call and in the backward pass."""
+    m, x = _block(), _gpu(_rand(1, 3, 20, 24))
+    params = list(m.parameters())
+    first, state = m(x[:, :9], return_state=True)
+    with pytest.raises(ValueError, match='detached'):
+        m(x[:, 9:], state=state)
+    with pytest.raises(RuntimeError, match='no gradient is computed for the state'):
+        torch.autograd.grad(state[0].sum(), params[0], retain_graph=True)
+    state = [s.detach() for s in state]
+    second = m(x[:, 9:], state=state)
+    with torch.no_grad():
+        assert torch.allclose(torch.cat([first, second], 1), m(x), rtol=1e-5, atol=1e-5)
+    together = torch.autograd.grad(first.sum() + second.sum(), params, retain_graph=True)
+    apart = [torch.autograd.grad(y.sum(), params) for y in (first, second)]
+    # the engine adds the same two terms, in fp32
+    assert all(torch.equal(t, a + b) for t, a, b in zip(together, *apart))

@@ -49,3 +49,48 @@ def test_operands_with_a_tangent_are_refused(name):
                 call(**dual)
     with pytest.raises(Launched):
         call(**args)
+
+
+def _returned_state(monkeypatch, x, w):
+    monkeypatch.setattr(ops, '_run', lambda *args: None)
+    return ops.causal_conv(x, w, return_state=True)
+
+
+def test_the_convolutions_state_passes_no_gradient_on_unnoticed(monkeypatch):
+    """The state that a call returns depends on its rows.  No gradient is computed for a state, so one that has not been
+    detached is refused by the next call, and a gradient of it by the backward pass, instead of being left out."""
+    x, w = torch.ones(6, 8, requires_grad=True), torch.ones(8, 4, requires_grad=True)
+    y, state = _returned_state(monkeypatch, x, w)
+    assert state.requires_grad
+    with pytest.raises(ValueError, match='detach'):
+        ops.causal_conv(x, w, state=state)
+    with pytest.raises(RuntimeError, match='no gradient is computed for the state'):
+        torch.autograd.grad(y.sum() + state.sum(), x)
+    ops.causal_conv(x, w, state=state.detach())
+    with torch.no_grad():                                 # nothing is left out where no gradient is wanted
+        ops.causal_conv(x, w, state=state)
+
+
+@pytest.mark.parametrize('x_grad,taps', [(False, 4), (True, 1)])
+def test_a_state_that_depends_on_no_leaf_needs_no_detaching(monkeypatch, x_grad, taps):
+    """Rows that are data, or one tap, whose state is empty."""
+    x, w = torch.ones(6, 8, requires_grad=x_grad), torch.ones(8, taps, requires_grad=True)
+    y, state = _returned_state(monkeypatch, x, w)
+    assert y.requires_grad and not state.requires_grad
+    ops.causal_conv(x, w, state=state)
+
+
+def test_block_refuses_a_state_of_its_own_that_is_not_detached(monkeypatch):
+    """Training in segments: with the window's share missing, the gradient would be neither the whole one nor the one that
+    is cut at the segments' border."""
+    from ps_vae_amd import modules
+    monkeypatch.setattr(ops, '_run', lambda *args: None)
+    monkeypatch.setattr(ops, 'linear', torch.nn.functional.linear)
+    m, x = modules.SSMBlock(8), torch.ones(2, 5, 8)
+    y, state = m(x, return_state=True)
+    with pytest.raises(ValueError, match='detached'):
+        m(x, state=state)
+    m(x, state=[s.detach() for s in state])
+    m(x, state=(state[0].detach(), state[1]))             # the scan's state by itself carries its whole gradient
+    with torch.no_grad():
+        m(x, state=state)
