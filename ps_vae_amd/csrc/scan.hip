@@ -199,6 +199,15 @@ template <int K> __device__ __forceinline__ void put_state(float* p, const float
     for (int k = 0; k < K; ++k) p[k] = h[k];
 }
 
+// A state behind a piece: h 2^(2 v) + e, the decay in two halves as it may leave fp32's range where the product does not: h is
+// zero in front of the first input whatever the rates and steps behind it sum up to (infinity times zero would be NaN), and
+// what is left of a large h that fades below 2^-126 of itself is still a number.  From v = 127 on every normal h but zero
+// becomes infinite.
+__device__ __forceinline__ float join(float h, float v, float e) {
+    const float half = __builtin_amdgcn_exp2f(fminf(v, 127.f));
+    return fmaf(half * h, half, e);
+}
+
 // Rows that no sequence holds become zero (one more z-slice of the grid does it, where the caller asks for it).
 template <class T> __device__ __forceinline__ void zero_rows(void* out, int64_t ld, const Scan& q, const Place& w, int slots) {
     if (!out) return;
@@ -245,10 +254,10 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(Scan q) {
         if (!ENDS && live)
             for (int i = 0; i < chunk; ++i) {          // join the chunks in front: h = exp(A sum) h + end
                 const int64_t row = (int64_t)i * q.S + s;
-                const float ds = q.chunk_s[row * q.Dn + d];
+                const float half_ds = 0.5f * q.chunk_s[row * q.Dn + d];
                 const float* e = own_state<K>(q.chunk_h, row, q, NP, d, n0);
 #pragma unroll
-                for (int k = 0; k < K; ++k) h[k] = fmaf(__builtin_amdgcn_exp2f(ds * A2[k]), h[k], e[k]);
+                for (int k = 0; k < K; ++k) h[k] = join(h[k], half_ds * A2[k], e[k]);
             }
         const int64_t first = sq.begin + (int64_t)tiles.first * TILE, row = first + r, bc_row = first + TileBC<T, P, K, VEC>::row();
         const T *px = (const T*)q.x + row * q.ldx + w.c0 + c, *pt = (const T*)q.dt + row * q.lddt + w.c0 + c,
@@ -386,11 +395,15 @@ __global__ __launch_bounds__(256, CARRY ? 3 : 2) void scan_bwd_kernel(Scan q) {
         if (!CARRY && live)
             for (int i = q.chunks - 1; i > chunk; --i) {
                 const int64_t row = (int64_t)(i - 1) * q.S + s;
-                const float ds = q.chunk_s[row * q.Dn + d];
+                const float half_ds = 0.5f * q.chunk_s[row * q.Dn + d];
                 const float* e = own_state<K>(q.chunk_h, row, q, NP, d, n0);
 #pragma unroll
-                for (int k = 0; k < K; ++k) ag[k] = fmaf(__builtin_amdgcn_exp2f(ds * A2[k]), ag[k], e[k]);
+                for (int k = 0; k < K; ++k) ag[k] = join(ag[k], half_ds * A2[k], e[k]);
             }
+        // dhT has to be here now: a wait for it inside the tiles would be one for the rows fetched ahead, too (8 x 2048 x 2048
+        // forward + backward: 793 against 787 us)
+#pragma unroll
+        for (int k = 0; k < K; ++k) asm volatile("" : "+v"(ag[k]));
         const int64_t first = sq.begin + (int64_t)(tiles.last - 1) * TILE;     // the last tile's first row
         const int64_t row = first + r, bc_row = first + TileBC<T, P, K, VEC>::row();
         const T *px = (const T*)q.x + row * q.ldx + w.c0 + c, *pt = (const T*)q.dt + row * q.lddt + w.c0 + c,

@@ -705,3 +705,69 @@ def test_block_trained_in_segments_cuts_the_gradient_at_their_border():
     apart = [torch.autograd.grad(y.sum(), params) for y in (first, second)]
     # the engine adds the same two terms, in fp32
     assert all(torch.equal(t, a + b) for t, a, b in zip(together, *apart))
+
+
+def _scan_with(dt, A, chunks, **kw):
+    """(outputs by name, oracle's outputs) of a scan of 96 rows of one sequence, in `chunks` pieces; no softplus."""
+    from ps_vae_amd import _lib, ops
+    v = {k: q for k, q in kw.items() if k not in ('dy', 'dhT')} | dict(dt=dt, A=A)
+    d = {k: q.double() for k, q in kw.items()} | dict(dt=dt.double(), A=A.double())
+    want = SO.selective_scan(off=[0, 96], softplus=False, **d)
+    leaves = {k: _gpu(q, grad=True) for k, q in v.items()}
+    old = _lib.set_option('scan_chunks', chunks)
+    try:
+        y, last = ops.selective_scan(**leaves, softplus=False, return_state=True)
+        grads = torch.autograd.grad((y, last), list(leaves.values()), (_gpu(kw['dy']), _gpu(kw['dhT'])))
+    finally:
+        _lib.set_option('scan_chunks', old)
+    names = dict(x='dx', dt='ddt', A='dA', B='dB', C='dC', h0='dh0')
+    return {'y': y, 'hT': last, **{names[k]: g for k, g in zip(leaves, grads)}}, want
+
+
+# The pieces of 96 rows are 32 rows each.  A piece's decay as a whole is exp of a sum of 32 steps, whose argument of size m
+# is off by m 2^-24 a step's rounding; rows one by one have the same.  13 roundings a row as for every scan above, and as
+# many again for larger arguments (three rows of 30, three roundings each; 3.5 elsewhere), once for the state and twice for a
+# gradient.
+_PIECES_C, _PIECES_C_GRAD = 2 * 13 * 96 + 32, 4 * 13 * 96 + 64
+
+
+@pytest.mark.parametrize('chunks', [1, 3])
+def test_growing_pieces_leave_a_state_of_zero_alone(chunks):
+    """Positive rates: a piece grows what enters it by more than fp32 holds (2^140 and more), but what enters is zero.  The
+    rows give finite values one by one, and so do the pieces, forward (no inputs before the second piece) and backward (no
+    gradients behind it)."""
+    rows, width, N = 96, 8, 4
+    A = 0.9 + 0.1 * torch.rand(width, N, generator=torch.Generator().manual_seed(1))
+    dt = torch.full((rows, width), 0.125)
+    dt[:32] = dt[64:] = 3.5                               # 32 x 3.5 x 0.9 = 101 and more: 145 bits
+    dt[32:35] = dt[61:64] = -30.0                         # what the middle passes on has lost 81 and more
+    middle = torch.zeros(rows, 1)
+    middle[35:61] = 1
+    args = dict(x=_rand(2, rows, width) * middle, dy=_rand(3, rows, width) * middle, B=_rand(4, rows, 1, N), C=_rand(5, rows, 1, N),
+                dhT=torch.zeros(1, width, N))
+    bits = (dt[:32].double()[..., None] * A.double()).sum(0) / 0.6931471805599453
+    assert float(bits.min()) > 128
+    got, want = _scan_with(dt, A, chunks, **args)
+    for k in got:
+        assert bool(got[k].isfinite().all()), k
+        _close(got[k], want[k], k, _PIECES_C if k in ('y', 'hT') else _PIECES_C_GRAD)
+
+
+@pytest.mark.parametrize('chunks', [1, 3])
+def test_fading_pieces_keep_what_is_left_of_a_large_state(chunks):
+    """A piece's decay below 2^-126 does not become zero in front of a state of 2^100: what is left of it is an ordinary
+    number.  The same backward with a large gradient of the last state."""
+    rows, width, N = 96, 8, 4
+    A = -(0.9 + 0.1 * torch.rand(width, N, generator=torch.Generator().manual_seed(1)))
+    zero, big = torch.zeros(rows, width), _rand(2, 1, width, N) * 2.0 ** 100
+    bc = dict(B=_rand(3, rows, 1, N), C=_rand(4, rows, 1, N))
+    dt = torch.full((rows, width), 0.125)
+    dt[:32] = 3.25                                        # 32 x 3.25 x 0.9 = 93 and more: 135 bits
+    got, want = _scan_with(dt, A, chunks, x=zero, dy=zero, h0=big, dhT=torch.zeros(1, width, N), **bc)
+    assert float(want['y'][0][32:].abs().min()) > 1e-20
+    for k in ('y', 'hT'):
+        _close(got[k], want[k], k, _PIECES_C)
+    got, want = _scan_with(dt.flip(0), A, chunks, x=zero, dy=zero, h0=torch.zeros(1, width, N), dhT=big, **bc)
+    assert float(want['dx'][0][:64].abs().min()) > 1e-20
+    for k in ('dx', 'dh0'):
+        _close(got[k], want[k], k, _PIECES_C_GRAD)
