@@ -189,6 +189,10 @@ class SSMBlock(nn.Module):
     def step(self, x, state):
         """x [S, dim]; `state` is moved on in place.  Returns the block's output rows."""
         window, h = state
+        # the convolution's part is moved on first: what the scan would refuse is refused before that
+        if h.shape != (x.shape[0], self.inner, self.num_states) or h.dtype != torch.float32 or h.device != x.device or not h.is_contiguous():
+            raise ValueError(f'SSMBlock: the state of the scan is {h.dtype} {tuple(h.shape)} on {h.device}, expected contiguous float32 '
+                             f'{(x.shape[0], self.inner, self.num_states)} on {x.device}')
         u, z = ops.linear(self.norm(x), self.in_proj.weight).chunk(2, dim=-1)
         v, _ = ops.causal_conv_step(u, window, self.conv_weight, self.conv_bias, silu=True)
         dt, B, C = self._split(v)

@@ -94,3 +94,20 @@ def test_block_refuses_a_state_of_its_own_that_is_not_detached(monkeypatch):
     m(x, state=(state[0].detach(), state[1]))             # the scan's state by itself carries its whole gradient
     with torch.no_grad():
         m(x, state=state)
+
+
+@pytest.mark.parametrize('spoil', [lambda h: h[:3], lambda h: h.half(), lambda h: h[..., :3].contiguous(), lambda h: h.transpose(0, 1).contiguous().transpose(0, 1)],
+                         ids=['sequences', 'type', 'states', 'order'])
+def test_block_step_moves_both_parts_of_a_state_or_neither(monkeypatch, spoil):
+    """A scan state that is refused is refused before the convolution's part has been moved on in place."""
+    from ps_vae_amd import modules
+    calls = []
+    monkeypatch.setattr(ops, '_run', lambda what, *args: calls.append(what))
+    monkeypatch.setattr(ops, 'linear', torch.nn.functional.linear)
+    m = modules.SSMBlock(8, num_states=4)
+    window, h = m.init_state(5)
+    with pytest.raises(ValueError, match='state'):
+        m.step(torch.ones(5, 8), (window, spoil(h)))
+    assert 'psvae_causal_conv_step' not in calls
+    m.step(torch.ones(5, 8), (window, h))
+    assert calls[-2:] == ['psvae_causal_conv_step', 'psvae_selective_scan_step']
