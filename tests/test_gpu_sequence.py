@@ -771,3 +771,77 @@ def test_fading_pieces_keep_what_is_left_of_a_large_state(chunks):
     assert float(want['dx'][0][:64].abs().min()) > 1e-20
     for k in ('dx', 'dh0'):
         _close(got[k], want[k], k, _PIECES_C_GRAD)
+
+
+class _Fenced:
+    """Tensors in the middle of larger ones: inputs between NaN, outputs between sevens that have to stay."""
+
+    def __init__(self, t):
+        self.t, self.outs = t, []
+
+    def _place(self, shape, value, dtype):
+        n = 1
+        for s in shape:
+            n *= s
+        pool = torch.full((n + 2 * 4096,), value, device=DEV, dtype=dtype)
+        return pool, pool[4096:4096 + n].view(shape)
+
+    def input(self, v, dtype=None):
+        pool, mid = self._place(v.shape, float('nan'), dtype or self.t)
+        mid.copy_(v)
+        return mid
+
+    def output(self, *shape, dtype=None):
+        pool, mid = self._place(shape, 7.0, dtype or self.t)
+        self.outs.append((pool, mid))
+        return mid
+
+    def check(self, what):
+        torch.cuda.synchronize()
+        for i, (pool, mid) in enumerate(self.outs):
+            assert bool((pool[:4096] == 7).all()) and bool((pool[4096 + mid.numel():] == 7).all()), (what, i, 'fence')
+            assert bool(mid.isfinite().all()), (what, i, 'a row from outside came in')
+
+
+@pytest.mark.parametrize('flag', [0, 4])
+@pytest.mark.parametrize('kind,D,N,W', [('f32', 8, 4, 4), ('bf16', 37, 5, 8), ('f16', 64, 33, 3)])
+@pytest.mark.parametrize('bad', [[0, 100, 200], [50, 60, 70], [30, 10, 40], [-5, 3, 1 << 30], [2 ** 31 - 1, -2 ** 31, 20], [39, 40, 39]], ids=str)
+def test_no_access_leaves_the_rows_whatever_the_offsets_hold(bad, kind, D, N, W, flag):
+    """Convolution and scan, forward, backward and states, in one piece and in three: nothing around any output changes, and
+    nothing around any input (NaN there) reaches a value.  What the values are is left open."""
+    import ctypes as C
+    from ps_vae_amd import _lib
+    L, st, t, f32 = _lib.lib(), torch.cuda.current_stream().cuda_stream, TYPES[kind], torch.float32
+    T, S, G, code = 40, 2, 1, {'f32': 0, 'bf16': 1, 'f16': 2}[kind]
+    assert flag in (0, _lib.SEQ_ZERO_OUTSIDE)
+    for chunks in (1, 3):
+        f = _Fenced(t)
+        x, dt, z, dy = (f.input(_rand(i, T, D)) for i in range(4))
+        B, Cm = (f.input(_rand(4 + i, T, G * N)) for i in range(2))
+        A, h0, dhT = f.input(-_rand(6, D, N).abs(), f32), f.input(_rand(7, S, D, N), f32), f.input(_rand(8, S, D, N), f32)
+        w, vec, state = f.input(_rand(9, D, W), f32), f.input(_rand(10, D), f32), f.input(_rand(11, S, W - 1, D))
+        off = torch.tensor([-7] + bad + [1 << 30], dtype=torch.int32, device=DEV)[1:4]
+        y, dx, ddt, dz, yc, dxc = (f.output(T, D) for _ in range(6))
+        dB, dC = f.output(T, G * N), f.output(T, G * N)
+        dA, dD, dbias, hT, dh0 = f.output(D, N, dtype=f32), f.output(D, dtype=f32), f.output(D, dtype=f32), f.output(S, D, N, dtype=f32), f.output(S, D, N, dtype=f32)
+        dw, db, state_out = f.output(D, W, dtype=f32), f.output(D, dtype=f32), f.output(S, W - 1, D)
+        old = _lib.set_option('scan_chunks', chunks)
+        try:
+            sizes = [L.psvae_selective_scan_saved_bytes(T, S, D, G, N), L.psvae_selective_scan_scratch_bytes(T, S, D, G, N, 0),
+                     L.psvae_selective_scan_scratch_bytes(T, S, D, G, N, 1), L.psvae_causal_conv_scratch_bytes(T, D, W, code)]
+            assert all(n % 4 == 0 for n in sizes) and (sizes[1] > 0) == (chunks > 1)
+            kept, fwd, bwd, conv = (f.output(n // 4, dtype=f32) for n in sizes)
+            a = _lib.Scan(x=x.data_ptr(), dt=dt.data_ptr(), B=B.data_ptr(), C=Cm.data_ptr(), z=z.data_ptr(), ldx=D, lddt=D, ldb=G * N, ldc=G * N, ldz=D,
+                          A=A.data_ptr(), skip=vec.data_ptr(), dt_bias=vec.data_ptr(), h0=h0.data_ptr(), seq_off=off.data_ptr(), T=T, S=S, D=D, G=G, N=N,
+                          dtype=code, flags=_lib.SEQ_SOFTPLUS | flag)
+            g = _lib.ScanGrads(dx=dx.data_ptr(), ddt=ddt.data_ptr(), dB=dB.data_ptr(), dC=dC.data_ptr(), dz=dz.data_ptr(), dA=dA.data_ptr(),
+                               d_skip=dD.data_ptr(), d_dt_bias=dbias.data_ptr(), dh0=dh0.data_ptr())
+            _lib.check(L.psvae_selective_scan_forward(C.byref(a), y.data_ptr(), D, hT.data_ptr(), kept.data_ptr(), fwd.data_ptr(), sizes[1], st))
+            _lib.check(L.psvae_selective_scan_backward(C.byref(a), kept.data_ptr(), dy.data_ptr(), D, dhT.data_ptr(), C.byref(g), bwd.data_ptr(), sizes[2], st))
+        finally:
+            _lib.set_option('scan_chunks', old)
+        _lib.check(L.psvae_causal_conv_forward(x.data_ptr(), D, w.data_ptr(), vec.data_ptr(), yc.data_ptr(), D, off.data_ptr(), state.data_ptr(),
+                                               state_out.data_ptr(), T, S, D, W, code, _lib.SEQ_SILU | flag, st))
+        _lib.check(L.psvae_causal_conv_backward(dy.data_ptr(), D, x.data_ptr(), D, w.data_ptr(), vec.data_ptr(), dxc.data_ptr(), D, dw.data_ptr(), db.data_ptr(),
+                                                off.data_ptr(), state.data_ptr(), T, S, D, W, code, _lib.SEQ_SILU | flag, conv.data_ptr(), sizes[3], st))
+        f.check((chunks, flag))
