@@ -410,7 +410,7 @@ def causal_conv_step(x, state, weight, bias=None, *, silu=False, state_out=None)
     S, D = x.shape
     weight, bias = _conv_params(what, x, weight, bias)
     _no_tangent(what, x, state, weight, bias, state_out)
-    if _wants_grad(x, state, weight, bias):
+    if _wants_grad(x, state, weight, bias, state_out):
         raise RuntimeError(f'{what} has no backward pass: call it under torch.no_grad() or on detached tensors')
     _act(what, 'state', state, x, (S, weight.shape[1] - 1, D))
     out = _state_out(what, state, state_out)
@@ -556,7 +556,7 @@ def selective_scan_step(x, dt, A, B, C, state, *, D=None, z=None, dt_bias=None, 
     if state.dtype != torch.float32:
         raise ValueError(f'{what}: state is {state.dtype}, expected torch.float32')
     _no_tangent(what, x, dt, A, B, C, state, D, z, dt_bias, state_out)
-    if _wants_grad(x, dt, A, B, C, state, D, z, dt_bias):
+    if _wants_grad(x, dt, A, B, C, state, D, z, dt_bias, state_out):
         raise RuntimeError(f'{what} has no backward pass: call it under torch.no_grad() or on detached tensors')
     out = _state_out(what, state, state_out)
     A, D, dt_bias, state, G = _scan_operands(what, x, dt, A, B, C, D, z, dt_bias, state, S)

@@ -111,3 +111,15 @@ def test_block_step_moves_both_parts_of_a_state_or_neither(monkeypatch, spoil):
     assert 'psvae_causal_conv_step' not in calls
     m.step(torch.ones(5, 8), (window, h))
     assert calls[-2:] == ['psvae_causal_conv_step', 'psvae_selective_scan_step']
+
+
+@pytest.mark.parametrize('name', ['causal_conv_step', 'selective_scan_step'])
+def test_token_steps_refuse_every_operand_that_requires_a_gradient(name):
+    """`state_out` too: it would go on requiring a gradient, with values that have no history."""
+    call, args = _operands()[name]
+    for k, v in args.items():
+        wants = {**args, k: v.clone().requires_grad_()}
+        with pytest.raises(RuntimeError, match='no backward pass'):
+            call(**wants)
+        with torch.no_grad(), pytest.raises(Launched):
+            call(**wants)
