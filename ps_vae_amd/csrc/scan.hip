@@ -400,10 +400,9 @@ __global__ __launch_bounds__(256, CARRY ? 3 : 2) void scan_bwd_kernel(Scan q) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) ag[k] = join(ag[k], half_ds * A2[k], e[k]);
             }
-        // dhT has to be here now: a wait for it inside the tiles would be one for the rows fetched ahead, too (8 x 2048 x 2048
-        // forward + backward: 793 against 787 us)
-#pragma unroll
-        for (int k = 0; k < K; ++k) asm volatile("" : "+v"(ag[k]));
+        // Wait for every load (vmcnt 0), dhT's above all: a wait for it inside the tiles would be one for the rows fetched ahead,
+        // too.  8 x 2048 x 2048 forward + backward 784 against 793 us without it, 32 x 512 x 2048 621 against 629.
+        __builtin_amdgcn_s_waitcnt(0x0f70);
         const int64_t first = sq.begin + (int64_t)(tiles.last - 1) * TILE;     // the last tile's first row
         const int64_t row = first + r, bc_row = first + TileBC<T, P, K, VEC>::row();
         const T *px = (const T*)q.x + row * q.ldx + w.c0 + c, *pt = (const T*)q.dt + row * q.lddt + w.c0 + c,
