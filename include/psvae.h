@@ -84,7 +84,8 @@ enum {
  *   gru_tiles      1 / 2 / 4: sequence tiles a workgroup of the multi-CU recurrence steps together
  *   gru_spin_ticks bound of a wait inside the multi-CU recurrence in ticks of 10 ns (default 2 s); 0: give up at
  *                  once, which exercises the redo on the single-CU kernels
- *   scan_chunks    1 .. 64: pieces of the time axis that the selective scan runs beside each other
+ *   scan_chunks    1 .. 64: pieces of the time axis that the selective scan runs beside each other; the library's choice
+ *                  takes every sequence for one of the mean length
  * psvae_option_set / _get return PSVAE_E_SHAPE for an unknown name; psvae_option_name(i) enumerates the names
  * (NULL past the last). */
 int psvae_option_set(const char* name, int value);

@@ -12,8 +12,10 @@
 // forming delta A with the 4 x 4 x 1 matrix instruction cost more in waits than it saved: 159 against 146 us): 3 vector
 // operations and one exponential, which takes twice as long, for the state, one for y; backward 15 and one exponential.
 // With the sums, softplus and gates a forward pass issues 8.3 vector instructions a cell, a backward pass 25, and counters
-// show the vector units busy 93 % and 87 % of the time.  Measured at 16 states, bf16, 32 x 512 x 2048 (0.54 G cells): 146 us
-// forward (1.8 TB/s of its 4 operands) and 468 us backward; HBM alone would take 54 and 110 us.
+// show the vector units busy 94 % and 86 % of the time.  Measured at 16 states, bf16, 32 x 512 x 2048 (0.54 G cells): forward
+// 142 us (1.9 TB/s of its 4 operands), backward 464 us.  HBM alone would take 54 us forward, 108 where the states are kept for
+// a backward pass (268 MB more; the kernel takes 155 us then), and 162 us backward (805 MB: 4 operands, the kept states, 3
+// gradients and the parts of dB and dC).
 //
 // Layout: P lanes side by side share a channel and hold K states each (P K = the states rounded up: 4 x 1, 4 x 2, 4 x 4,
 // 8 x 4, 16 x 4), a workgroup of 256 lanes takes 256 / P channels of one group and one sequence and walks the time axis in
@@ -770,10 +772,16 @@ Plan scan_plan(int64_t T, int S, int D, int G, int N) {
     p.tiles = (D / G + p.CB - 1) / p.CB;
     p.blocks = p.tiles * G;
     // Chunks: the two-pass form computes every exponential twice, so it is taken only where workgroups of whole sequences are
-    // fewer than two for every CU (16 x 1024 x 2048, 16 states: 512 workgroups in one piece 174 + 480 us forward + backward,
-    // in two 205 + 537; 12 x 1365: 384 in one piece 229 + 631, in four 227 + 554).  Then there are four for every CU at least,
-    // as near above a whole number of them as 5 % where twice as many pieces reach that (12 x 1365: three pieces make 4.5 for
-    // every CU and take 233 + 593), and a piece has four tiles on average.
+    // fewer than two for every CU (16 x 1024 x 2048, 16 states: 512 workgroups in one piece 174 us forward, 673 a training pass;
+    // in two 202 and 747).  Then there are four for every CU at least, as near above a whole number of them as 5 % where twice
+    // as many pieces reach that, and a piece has four tiles on average.  Prompt and training pass in us, * the rule's choice:
+    //   12 x 1365 x 2048 (384 workgroups): one piece 230 and 878, two 230 and 823, three 229 and 838, four* 221 and 788, six 221 and 790
+    //   8 x 2048 x 2048 (256): one 282 and 974, two 260 and 849, three 229 and 821, four* 222 and 789, six 219 and 780, eight 220 and 794
+    //   4 x 4096 x 2048 (128): four 288 and 908, eight* 243 and 832, sixteen 232 and 821, thirty-two 239 and 865
+    //   5 x 1024 x 1004, 64 states (315): one 159 and 631, three 136 and 518, four* 126 and 498, six 131 and 523, eight 126 and 511
+    // The host knows the number of sequences and rows and not the lengths, so every sequence counts as one of the mean length: a
+    // long one among many short ones is walked in too few pieces (8191 rows and 100 of 30, width 512: one piece 1094 and 3634,
+    // sixteen 337 and 953); the option scan_chunks helps a caller who knows them.
     const int64_t whole = (int64_t)p.blocks * (S > 0 ? S : 1), tiles = (T + TILE - 1) / TILE;
     int64_t c = 1;
     if (whole < 512) {

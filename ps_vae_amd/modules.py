@@ -121,7 +121,8 @@ class LayerNorm(nn.LayerNorm):
 
 class SSMBlock(nn.Module):
     """A pre-norm state-space block over sequences, the recurrent layer for long sequences beside the decoder's GRU (no
-    counterpart in the reference):
+    counterpart in the reference).  Its layers, and how A_log, D and dt_proj's bias begin, are those of the published selective
+    state-space block (A. Gu and T. Dao, 2023), so that weights of such a block have a place here:
 
         u, z = in_proj(norm(x));  v = silu(causal_conv(u));  r, B, C = x_proj(v)
         out = x + out_proj(selective_scan(v, dt_proj(r), -exp(A_log), B, C, D, gate z))
