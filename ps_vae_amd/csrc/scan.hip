@@ -203,8 +203,8 @@ template <int K> __device__ __forceinline__ void put_state(float* p, const float
 
 // A state behind a piece: h 2^(2 v) + e, the decay in two halves as it may leave fp32's range where the product does not: h is
 // zero in front of the first input whatever the rates and steps behind it sum up to (infinity times zero would be NaN), and
-// what is left of a large h that fades below 2^-126 of itself is still a number.  From v = 127 on every normal h but zero
-// becomes infinite.
+// what is left of a large h that fades below 2^-126 of itself is still a number.  From v = 127 on every normal h
+// becomes infinite, and zero stays zero.
 __device__ __forceinline__ float join(float h, float v, float e) {
     const float half = __builtin_amdgcn_exp2f(fminf(v, 127.f));
     return fmaf(half * h, half, e);
